@@ -429,6 +429,84 @@ int ctct_b200_profile_enable(int max_calls);
 int ctct_b200_profile_read(float *ms, int *kind, int capacity);
 int ctct_b200_profile_disable(void);
 
+/* ---------------------------------------------------------------------------------------------
+ * Operators of the joiner, before the loss.  No counterpart in the reference, whose callers build the
+ * joint tensor themselves (warp_ctct/__init__.py:97-100).
+ * ------------------------------------------------------------------------------------------- */
+
+/*
+ * Layer norm over the last dimension of `rows` rows of H elements (x: `x_stride` elements from row to row,
+ * the elements of a row adjacent; y contiguous):
+ *   y = (x - mean) / sqrt(variance + eps) * weight + bias
+ * weight, bias (H) or NULL (1 and 0), float32 if param_f32, else of `dtype`.  Sums are float32; the one
+ * rounding is that of y.  stats: 2 * rows floats out {mean, 1/deviation} for the backward pass, or NULL.
+ * Backward: dx (rows, H) contiguous, dweight, dbias (H, type of the weight), each may be NULL; workspace of
+ * ctct_b200_layer_norm_workspace_bytes, needed for dweight or dbias only.  No atomics: the same bits
+ * every time.
+ */
+size_t ctct_b200_layer_norm_workspace_bytes(int64_t rows, int64_t H, int dtype);
+int ctct_b200_layer_norm_forward(const void *x, int64_t x_stride, int dtype, int64_t rows, int64_t H, const void *weight,
+                                 const void *bias, int param_f32, float eps, void *y, float *stats, void *stream);
+int ctct_b200_layer_norm_backward(const void *dy, int64_t dy_stride, const void *x, int64_t x_stride, int dtype,
+                                  int64_t rows, int64_t H, const void *weight, int param_f32, const float *stats, void *dx,
+                                  void *dweight, void *dbias, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Layer norm of an additive joiner: y[n,t,u] = layer_norm(f[n,t] + g[n,u]) over H, without the sum in memory.
+ *   f (N,T,H), g (N,U1,H): strides in elements (f_sn, f_st; g_sn, g_su), the elements of a row adjacent
+ *   packed_rows < 0: y (N,T,U1,H); frames t >= lx[n] and contexts u > ly[n] are written as zeros; lx, ly may be
+ *     NULL (every frame, every label)
+ *   packed_rows >= 0: y (packed_rows, H), the packed layout of ctct_b200_loss_forward_packed; rows that the lengths
+ *     place beyond packed_rows are not written, rows behind the last utterance are written as zeros
+ *   saved: ctct_b200_joint_norm_saved_bytes, 256-byte aligned, kept for the backward pass (want_grad); without
+ *     want_grad only the packed layout needs it (0 bytes otherwise: may be NULL)
+ * Lengths outside [0, T] and [0, U1 - 1] are clamped.  H up to CTCT_MAX_JOINT_H.
+ * Backward: dy of y's shape, contiguous (its padding is not read); df (N,T,H), dg (N,U1,H) contiguous, of `dtype`,
+ * zeros where no valid row is; dweight, dbias (H); each may be NULL.
+ */
+#define CTCT_MAX_JOINT_H 16384
+size_t ctct_b200_joint_norm_saved_bytes(int64_t N, int64_t T, int64_t U1, int64_t packed_rows, int want_grad);
+size_t ctct_b200_joint_norm_workspace_bytes(int64_t N, int64_t T, int64_t U1, int64_t H);
+int ctct_b200_joint_norm_forward(const void *f, int64_t f_sn, int64_t f_st, const void *g, int64_t g_sn, int64_t g_su,
+                                 int dtype, const int32_t *lx, const int32_t *ly, int64_t N, int64_t T, int64_t U1,
+                                 int64_t H, int64_t packed_rows, const void *weight, const void *bias, int param_f32,
+                                 float eps, void *y, int want_grad, void *saved, size_t saved_bytes, void *stream);
+int ctct_b200_joint_norm_backward(const void *dy, const void *f, int64_t f_sn, int64_t f_st, const void *g, int64_t g_sn,
+                                  int64_t g_su, int dtype, const int32_t *lx, const int32_t *ly, int64_t N, int64_t T,
+                                  int64_t U1, int64_t H, int64_t packed_rows, const void *weight, int param_f32,
+                                  const void *saved, size_t saved_bytes, void *df, void *dg, void *dweight, void *dbias,
+                                  void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Adjustment of raw logits: for token v with c occurrences in the row's history
+ *   z = x;  c > 0: z = x > 0 ? x / repetition : x * repetition;  z -= presence * [c > 0] + frequency * c;
+ *   z += bias[v];  out = allowed(v) ? z : -inf
+ * Rows: (N,T,U1,V) with lx, ly or NULL (padding rows are written as zeros); packed_rows >= 0: (packed_rows, V) as above,
+ * cu_rows (N + 1) int64 is filled in by the forward call and read by the backward call; a decoder's step is
+ * T = U1 = 1, where row_stride > 0 gives the elements from row to row of `logits` (0: contiguous).
+ *   tokens: histories, `tokens_pitch` entries per n.  tokens_lengths (N): all rows of n have the first
+ *     tokens_lengths[n]; NULL: context u has the first u (labels).  Entries outside [0, V) are ignored.  NULL: none
+ *   bias_kind, mask_kind: 0 none, 1 shared (V), 2 per n (N,V), 3 per context (N,U1,V).  bias: float32 if bias_f32, else
+ *     of `dtype`.  allowed: bit v % 32 of word v / 32, rows of ceil(V / 32) words
+ *   repetition > 0, presence, frequency: for all rows, unless the pointer to (N) floats of the same name is given
+ * Masked places are -inf whatever stood there.  Backward: dx (shape and type of out) and dbias (shape and type of
+ * bias), each may be NULL; `logits` is read only where a repeated token is scaled (NULL if repetition is 1 for all
+ * rows); dy is not read in padding rows, masked places get zero.  workspace: ctct_b200_adjust_workspace_bytes, for dbias only.
+ */
+size_t ctct_b200_adjust_workspace_bytes(int64_t N, int64_t T, int64_t U1, int64_t V);
+int ctct_b200_adjust_forward(const void *logits, int64_t row_stride, int dtype, const int32_t *tokens, int64_t tokens_pitch,
+                             const int32_t *tokens_lengths, const int32_t *lx, const int32_t *ly, int64_t N, int64_t T,
+                             int64_t U1, int64_t V, int64_t packed_rows, int64_t *cu_rows, const void *bias, int bias_kind,
+                             int bias_f32, const int32_t *allowed, int mask_kind, float repetition, float presence,
+                             float frequency, const float *repetition_n, const float *presence_n,
+                             const float *frequency_n, void *out, void *stream);
+int ctct_b200_adjust_backward(const void *dy, const void *logits, int64_t row_stride, int dtype, const int32_t *tokens,
+                              int64_t tokens_pitch, const int32_t *tokens_lengths, const int32_t *lx, const int32_t *ly,
+                              int64_t N, int64_t T, int64_t U1, int64_t V, int64_t packed_rows, const int64_t *cu_rows,
+                              int bias_kind, int bias_f32, const int32_t *allowed, int mask_kind, float repetition,
+                              const float *repetition_n, void *dx, void *dbias, void *workspace, size_t workspace_bytes,
+                              void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -329,6 +329,9 @@ def ctct_loss_and_grad(log_probs: T, labels: T, frames_lengths: T, labels_length
     return loss, _fused_backward(ctx, seed)
 
 
+from .adjust import (AdjustLogits, adjust_joint_logits, adjust_joint_logits_packed, adjust_logits,  # noqa: E402,F401
+                     pack_token_mask)
+from .layernorm import JointLayerNorm, LayerNorm, joint_layer_norm, joint_layer_norm_packed, layer_norm  # noqa: E402,F401
 from .logits import FusedLogitsCTCTLoss, FusedLogitsCTCTLossReduced, ctct_loss_from_logits  # noqa: E402,F401
 from .packed import FusedPackedCTCTLoss, ctct_loss_packed, pack_joint, unpack_joint  # noqa: E402,F401
 from .simple import (FusedSimpleCTCTLoss, LogMMExp, SimpleCTCTLoss, ctct_loss_simple_fwd,  # noqa: E402,F401

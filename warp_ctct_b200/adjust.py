@@ -1,0 +1,271 @@
+"""Adjustment of raw logits: penalties for repeated tokens, additive biases, masks of allowed tokens.
+
+For a token v that occurs c times in the history of a row with logit x::
+
+    z = x;  if c > 0: z = x / repetition_penalty if x > 0 else x * repetition_penalty
+    z -= presence_penalty * (c > 0) + frequency_penalty * c
+    z += bias[v]
+    out = z if v is allowed else -inf
+
+``adjust_logits`` is the step of a decoder: (R, V) logits, a history per row.  ``adjust_joint_logits`` and
+``adjust_joint_logits_packed`` do the same to every row of a joint tensor before ``ctct_loss_from_logits`` or
+``ctct_loss_packed(from_logits=True)`` (the reference takes the joint tensor as it is, warp_ctct/__init__.py:97-100): the
+history of a row is its context's labels.  Gradients flow to the logits and to the bias.
+"""
+from __future__ import annotations
+
+from typing import Optional, Union
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+T = torch.Tensor
+
+
+def pack_token_mask(mask: T) -> T:
+    """(..., V) truth values -> (..., ceil(V / 32)) int32 words, bit v % 32 of word v // 32: the ``allowed`` argument of
+    the functions below."""
+    V = mask.size(-1)
+    words = (V + 31) // 32
+    bits = torch.nn.functional.pad(mask.to(torch.int64), (0, words * 32 - V)).view(*mask.shape[:-1], words, 32)
+    packed = (bits << torch.arange(32, device=mask.device)).sum(-1)
+    return torch.where(packed >= 1 << 31, packed - (1 << 32), packed).to(torch.int32)
+
+
+class _Call:
+    """The arguments of one adjustment, checked: what the C entry points of both directions take."""
+
+    __slots__ = ("N", "T", "U1", "V", "rows", "row_stride", "tokens", "pitch", "lengths", "lx", "ly", "cu", "bias_kind", "bias_dtype",
+                 "allowed", "mask_kind", "scalars", "tensors")
+
+
+def _penalty(name: str, value: Union[float, T], N: int, device, positive: bool):
+    """(scalar, tensor or None) of a penalty given as a number or as (N,) float32."""
+    if not isinstance(value, torch.Tensor):
+        value = float(value)
+        if not (value > 0.0 if positive else value == value) or value in (float("inf"), float("-inf")):
+            raise RuntimeError(f"{name} must be a finite number{' above 0' if positive else ''}, not {value}")
+        return value, None
+    if value.dim() != 1 or value.size(0) != N:
+        raise RuntimeError(f"{name} must be a number or have shape ({N},)")
+    if value.dtype != torch.float32 or value.device != device:
+        raise RuntimeError(f"{name} must be float32 on {device}")
+    if value.requires_grad:
+        raise RuntimeError(f"{name} is not differentiated: detach it")
+    return 1.0, value.contiguous()
+
+
+def _kind(name: str, t: Optional[T], N: int, U1: int, last: int, step: bool, device) -> int:
+    """0 none, 1 (last), 2 (N, last), 3 (N, U1, last)."""
+    if t is None:
+        return 0
+    if t.device != device:
+        raise RuntimeError(f"{name} must be on {device}, not on {t.device}")
+    for kind, shape in ((1, (last,)), (2, (N, last)), (3, (N, U1, last))):
+        if tuple(t.shape) == shape and not (step and kind == 3):
+            return kind
+    per_context = "" if step else f" or ({N}, {U1}, {last})"
+    raise RuntimeError(f"{name} must have shape ({last},), ({N}, {last}){per_context}, not {tuple(t.shape)}")
+
+
+def _prepare(logits: T, N: int, Tm: int, U1: int, rows: int, row_stride: int, tokens: Optional[T], pitch: int, lengths: Optional[T],
+             lx: Optional[T], ly: Optional[T], bias: Optional[T], allowed: Optional[T], repetition, presence, frequency, step: bool):
+    dev = logits.device
+    V = logits.size(-1)
+    if V < 1:
+        raise RuntimeError("logits must have at least one token")
+    c = _Call()
+    c.N, c.T, c.U1, c.V, c.rows, c.row_stride = N, Tm, U1, V, rows, row_stride
+    c.tokens, c.pitch, c.lengths, c.lx, c.ly, c.cu = tokens, pitch, lengths, lx, ly, None
+    c.bias_kind = _kind("bias", bias, N, U1, V, step, dev)
+    c.bias_dtype = None
+    if bias is not None:
+        if bias.dtype != logits.dtype and bias.dtype != torch.float32:
+            raise RuntimeError(f"bias must be float32 or of the logits' type {logits.dtype}, not {bias.dtype}")
+        c.bias_dtype = bias.dtype
+    c.mask_kind = _kind("allowed", allowed, N, U1, (V + 31) // 32, step, dev)
+    if allowed is not None and allowed.dtype != torch.int32:
+        raise RuntimeError("allowed must be int32 words (pack_token_mask)")
+    c.allowed = None if allowed is None else allowed.contiguous()
+    r, rn = _penalty("repetition_penalty", repetition, N, dev, True)
+    p, pn = _penalty("presence_penalty", presence, N, dev, False)
+    q, qn = _penalty("frequency_penalty", frequency, N, dev, False)
+    c.scalars, c.tensors = (r, p, q), (rn, pn, qn)
+    return c
+
+
+def _forward(c: _Call, logits: T, bias: Optional[T]) -> T:
+    dev = logits.device
+    with _lib.on_device(dev):
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        if c.rows >= 0:
+            c.cu = torch.empty((c.N + 1,), dtype=torch.int64, device=dev)
+        rn, pn, qn = c.tensors
+        rc = _lib.lib().ctct_b200_adjust_forward(
+            logits.data_ptr(), c.row_stride, _lib.dtype_code(logits.dtype), _lib.ptr(c.tokens), c.pitch, _lib.ptr(c.lengths),
+            _lib.ptr(c.lx), _lib.ptr(c.ly), c.N, c.T, c.U1, c.V, c.rows, _lib.ptr(c.cu), _lib.ptr(bias), c.bias_kind,
+            int(c.bias_dtype == torch.float32), _lib.ptr(c.allowed), c.mask_kind, *c.scalars, _lib.ptr(rn), _lib.ptr(pn),
+            _lib.ptr(qn), out.data_ptr(), _lib.raw_stream(dev))
+    _lib.check(rc, "ctct_b200_adjust_forward")
+    return out
+
+
+class AdjustLogits(torch.autograd.Function):
+    """Keeps the logits only if a repetition penalty scales some of them."""
+
+    @staticmethod
+    def forward(ctx, logits: T, bias: Optional[T], c: _Call):
+        out = _forward(c, logits, bias)
+        scaled = c.tokens is not None and (c.tensors[0] is not None or c.scalars[0] != 1.0)
+        # tensors that a caller could change in between go through save_for_backward, which notices
+        ctx.save_for_backward(logits if scaled else None, c.tokens, c.lengths, c.lx, c.ly, c.cu, c.allowed, c.tensors[0])
+        ctx.c, ctx.like = c, (logits.shape, logits.dtype, logits.device, None if bias is None else bias.shape)
+        c.tokens = c.lengths = c.lx = c.ly = c.cu = c.allowed = c.tensors = None
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy: T):
+        logits, tokens, lengths, lx, ly, cu, allowed, rn = ctx.saved_tensors
+        c, (shape, dtype, dev, bias_shape) = ctx.c, ctx.like
+        lib = _lib.lib()
+        dy = dy.contiguous()
+        need_x, need_b = ctx.needs_input_grad[:2]
+        with _lib.on_device(dev):
+            dx = torch.empty(shape, dtype=dtype, device=dev) if need_x else None
+            db = torch.empty(bias_shape, dtype=c.bias_dtype, device=dev) if need_b else None
+            ws, nbytes = None, 0
+            if need_b:
+                nbytes = lib.ctct_b200_adjust_workspace_bytes(c.N, c.T, c.U1, c.V)
+                ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+            rc = lib.ctct_b200_adjust_backward(
+                dy.data_ptr(), _lib.ptr(logits), c.row_stride, _lib.dtype_code(dtype), _lib.ptr(tokens), c.pitch,
+                _lib.ptr(lengths), _lib.ptr(lx), _lib.ptr(ly), c.N, c.T, c.U1, c.V, c.rows, _lib.ptr(cu), c.bias_kind,
+                int(c.bias_dtype == torch.float32), _lib.ptr(allowed), c.mask_kind, c.scalars[0], _lib.ptr(rn), _lib.ptr(dx),
+                _lib.ptr(db), _lib.ptr(ws), nbytes, _lib.raw_stream(dev))
+        _lib.check(rc, "ctct_b200_adjust_backward")
+        return dx, db, None
+
+
+def _apply(c: _Call, logits: T, bias: Optional[T]) -> T:
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    if torch.is_grad_enabled() and (logits.requires_grad or (bias is not None and bias.requires_grad)):
+        return AdjustLogits.apply(logits, bias, c)
+    return _forward(c, logits, bias)
+
+
+def _int_on(name: str, t: T, device) -> T:
+    from . import _as_int
+    if t.device != device:
+        raise RuntimeError(f"{name} must be on {device}, not on {t.device}")
+    if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
+        raise RuntimeError(f"{name} must hold integers, not {t.dtype}")
+    return _as_int(t)
+
+
+def adjust_logits(logits: T, tokens: Optional[T] = None, tokens_lengths: Optional[T] = None, bias: Optional[T] = None,
+                  allowed: Optional[T] = None, repetition_penalty: Union[float, T] = 1.0,
+                  presence_penalty: Union[float, T] = 0.0, frequency_penalty: Union[float, T] = 0.0) -> T:
+    """One decoding step: the adjusted logits of R rows.
+
+    Args:
+        logits: (R, V) float32, float16 or bfloat16 on the GPU; rows may be apart (``scores[:, -1]`` is read in place).
+        tokens: (R, L) integer history of every row (None: no history); entries outside [0, V) are ignored.
+        tokens_lengths: (R,) tokens of each history, the first ones of its row (None: all L).
+        bias: (V,) or (R, V), float32 or the logits' type.
+        allowed: (ceil(V/32),) or (R, ceil(V/32)) int32 words of allowed tokens (``pack_token_mask``).
+        repetition_penalty, presence_penalty, frequency_penalty: numbers, or (R,) float32 tensors.
+    Returns (R, V), contiguous, in the type of the logits; -inf where a token is not allowed.
+    """
+    if not logits.is_cuda:
+        raise RuntimeError("logits must be located in the CUDA")
+    _lib.dtype_code(logits.dtype)
+    if logits.dim() != 2:
+        raise RuntimeError("logits must have 2 dims.")
+    R, V = logits.shape
+    dev = logits.device
+    if (logits.stride(1) != 1 and V > 1) or logits.stride(0) < V:
+        logits = logits.contiguous()
+    if tokens is not None:
+        if tokens.dim() != 2 or tokens.size(0) != R:
+            raise RuntimeError(f"tokens must have shape ({R}, L)")
+        L = tokens.size(1)
+        tokens = _int_on("tokens", tokens, dev)
+        if tokens_lengths is None:
+            tokens_lengths = torch.full((R,), L, dtype=torch.int32, device=dev)
+        elif tokens_lengths.dim() != 1 or tokens_lengths.size(0) != R:
+            raise RuntimeError(f"tokens_lengths must have shape ({R},)")
+        else:
+            tokens_lengths = _int_on("tokens_lengths", tokens_lengths, dev)
+    elif tokens_lengths is not None:
+        raise RuntimeError("tokens_lengths without tokens")
+    else:
+        L = 0
+    c = _prepare(logits, R, 1, 1, -1, 0 if logits.is_contiguous() else logits.stride(0), tokens, L, tokens_lengths, None, None, bias,
+                 allowed, repetition_penalty, presence_penalty, frequency_penalty, True)
+    return _apply(c, logits, bias)
+
+
+def _joint_args(logits: T, labels: T, frames_lengths: Optional[T], labels_lengths: Optional[T]):
+    if not logits.is_cuda:
+        raise RuntimeError("logits must be located in the CUDA")
+    _lib.dtype_code(logits.dtype)
+    if labels.dim() != 2:
+        raise RuntimeError("labels must have 2 dims.")
+    N = labels.size(0)
+    for name, t in (("frames_lengths", frames_lengths), ("labels_lengths", labels_lengths)):
+        if t is not None and (t.dim() != 1 or t.size(0) != N):
+            raise RuntimeError(f"{name} must have shape ({N},)")
+    dev = logits.device
+    return (_int_on("labels", labels, dev), None if frames_lengths is None else _int_on("frames_lengths", frames_lengths, dev),
+            None if labels_lengths is None else _int_on("labels_lengths", labels_lengths, dev))
+
+
+def adjust_joint_logits(logits: T, labels: T, frames_lengths: Optional[T] = None, labels_lengths: Optional[T] = None,
+                        bias: Optional[T] = None, allowed: Optional[T] = None, repetition_penalty: Union[float, T] = 1.0,
+                        presence_penalty: Union[float, T] = 0.0, frequency_penalty: Union[float, T] = 0.0) -> T:
+    """The adjusted logits of a joint tensor, for ``ctct_loss_from_logits`` on the same labels and lengths.
+
+    Args:
+        logits: (N, T, U, V) raw scores, U = max labels + 1; float32, float16 or bfloat16.
+        labels: (N, U-1); the history of rows [n, :, u] is labels[n, :u].
+        frames_lengths, labels_lengths: (N,); rows beyond them are zeros and take no part in any gradient.
+            None: all rows are valid.
+        bias: (V,), (N, V) or (N, U, V), float32 or the logits' type.
+        allowed: (ceil(V/32),), (N, ceil(V/32)) or (N, U, ceil(V/32)) int32 words (``pack_token_mask``): a grammar's
+            state for each context.
+        repetition_penalty, presence_penalty, frequency_penalty: numbers, or (N,) float32 tensors.
+    """
+    labels, lx, ly = _joint_args(logits, labels, frames_lengths, labels_lengths)
+    if logits.dim() != 4 or logits.size(0) != labels.size(0) or logits.size(2) != labels.size(1) + 1:
+        raise RuntimeError("logits must have shape (N, T, U, V), labels (N, U - 1)")
+    logits = logits.contiguous()
+    N, Tm, U1, _ = logits.shape
+    c = _prepare(logits, N, Tm, U1, -1, 0, labels, U1 - 1, None, lx, ly, bias, allowed, repetition_penalty, presence_penalty,
+                 frequency_penalty, False)
+    return _apply(c, logits, bias)
+
+
+def adjust_joint_logits_packed(logits: T, labels: T, frames_lengths: T, labels_lengths: T, max_frames: Optional[int] = None,
+                               bias: Optional[T] = None, allowed: Optional[T] = None, repetition_penalty: Union[float, T] = 1.0,
+                               presence_penalty: Union[float, T] = 0.0, frequency_penalty: Union[float, T] = 0.0) -> T:
+    """``adjust_joint_logits`` on a packed (rows, V) joint tensor (``pack_joint``), for ``ctct_loss_packed(from_logits=True)``.
+
+    max_frames: an upper bound of frames_lengths known on the host; omitted, it is read back from the device (one
+    synchronisation).  Rows that the lengths place beyond the tensor are not touched, surplus rows are zeros.
+    """
+    labels, lx, ly = _joint_args(logits, labels, frames_lengths, labels_lengths)
+    if logits.dim() != 2:
+        raise RuntimeError("packed logits must have 2 dims.")
+    if max_frames is None:
+        max_frames = int(lx.max().item()) if lx.numel() else 0
+    if max_frames < 0:
+        raise RuntimeError("max_frames must not be negative")
+    logits = logits.contiguous()
+    U1 = labels.size(1) + 1
+    c = _prepare(logits, labels.size(0), int(max_frames), U1, logits.size(0), 0, labels, U1 - 1, None, lx, ly, bias, allowed,
+                 repetition_penalty, presence_penalty, frequency_penalty, False)
+    return _apply(c, logits, bias)

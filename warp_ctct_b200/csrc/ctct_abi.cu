@@ -9,6 +9,7 @@
 #include "gather.cuh"
 #include "grad.cuh"
 #include "lattice.cuh"
+#include "launch.cuh"
 #include "logits.cuh"
 #include "simple.cuh"
 #include "logmm_tc.cuh"
@@ -18,15 +19,17 @@
 using namespace ctct;
 
 namespace {
-
 thread_local char g_last_cuda_error[256] = "";
+}
 
-int check_launch(const char *what) {
+int ctct::check_launch(const char *what) {
     const cudaError_t err = cudaGetLastError();
     if (err == cudaSuccess) return CTCT_OK;
     snprintf(g_last_cuda_error, sizeof(g_last_cuda_error), "%s: %s", what, cudaGetErrorString(err));
     return CTCT_ERR_LAUNCH;
 }
+
+namespace {
 
 // ---- optional event recorder (benchmarks only) ----
 struct Profiler {
@@ -48,29 +51,6 @@ cudaEvent_t *prof_slot(int kind) {
 }
 inline void prof_mark(cudaEvent_t *slot, int i, cudaStream_t st) {
     if (slot) cudaEventRecord(slot[i], st);
-}
-
-// Launch with programmatic stream serialisation: the kernel may be set up, and start, while the
-// kernel before it in the stream drains; it must call pdl_wait() before touching that kernel's output.
-template <typename... KArgs, typename... Args>
-cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args &&...args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
-}
-
-int sm_count() {
-    int dev = 0, sms = 148;
-    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    return sms > 0 ? sms : 148;
 }
 
 // Lattice slots (two per context) per thread and threads per CTA.  One warp handles 32 slots;
@@ -111,8 +91,6 @@ bool lattice_config(int64_t U1, LatCfg *cfg) {
     }
     return false;
 }
-
-size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 struct WsLayout {
     size_t G, TAB, LLF, LLI, total;

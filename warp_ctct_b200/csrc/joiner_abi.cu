@@ -1,0 +1,570 @@
+// extern "C" entry points of the joiner's operators: layer norm, the additive joiner's layer norm, the
+// adjustment of logits (declared in include/ctct_b200.h).  Argument checks, choice of a kernel variant,
+// workspace carving and launches; nothing here allocates or synchronises.
+#include "../../include/ctct_b200.h"
+
+#include "adjust.cuh"
+#include "elem.cuh"
+#include "jointnorm.cuh"
+#include "launch.cuh"
+#include "layernorm.cuh"
+
+using namespace ctct;
+
+namespace {
+
+size_t esize(int dtype) { return dtype == CTCT_F32 ? 4 : 2; }
+bool dtype_ok(int dtype) { return dtype == CTCT_F32 || dtype == CTCT_F16 || dtype == CTCT_BF16; }
+bool aligned(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+// call fn(T{}) with the element type of a dtype code
+template <typename F>
+int with_type(int dtype, F &&fn) {
+    switch (dtype) {
+    case CTCT_F32: return fn(float{});
+    case CTCT_F16: return fn(__half{});
+    default: return fn(__nv_bfloat16{});
+    }
+}
+
+constexpr int64_t kMaxGrid = 0x7fffffff;
+constexpr int kSms = 148;  // SMs of a B200: grids and workspaces are sized by it
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// ---- layer norm ----
+// Elements of a row per thread: 8 up to 256 per row (a warp each), else 16; float32 rows stay at 8 as long as
+// 512 threads cover the row, since 16 float32 of x and dy and their successors do not fit 128 registers.
+int ln_elems(int64_t H, int dtype) { return H <= 256 || (dtype == CTCT_F32 && H <= 8 * LN_WIDE_THREADS) ? 8 : 16; }
+struct LnGeom {
+    int P;
+    bool wide, is_long;
+    int threads;
+    int64_t grid;
+};
+LnGeom ln_geom(int64_t rows, int64_t H, int dtype) {
+    LnGeom g;
+    g.P = ln_elems(H, dtype);
+    g.is_long = H > static_cast<int64_t>(g.P) * LN_WIDE_THREADS;
+    g.wide = H > 32 * g.P;
+    g.threads = g.is_long ? LN_WIDE_THREADS : g.wide ? static_cast<int>(ceil_div(H, 32 * g.P)) * 32 : 32 * LN_WARPS;
+    // resident blocks: 512 threads' worth per SM
+    const int64_t blocks = g.wide ? rows : ceil_div(rows, LN_WARPS);
+    const int64_t most = static_cast<int64_t>(kSms) * (512 / g.threads > 0 ? 512 / g.threads : 1);
+    g.grid = blocks < most ? blocks : most;
+    return g;
+}
+
+template <typename T, int VE, int P>
+void ln_launch(const LnGeom &g, const LnArgs &a, cudaStream_t st) {
+    const dim3 grid(static_cast<unsigned>(g.grid)), block(g.threads);
+    if (g.wide)
+        launch_pdl(k_ln_forward<T, VE, P, true>, grid, block, 0, st, a);
+    else
+        launch_pdl(k_ln_forward<T, VE, P, false>, grid, block, 0, st, a);
+}
+template <typename T, int VE, int P>
+void ln_launch(const LnGeom &g, const LnGradArgs &a, cudaStream_t st) {
+    const dim3 grid(static_cast<unsigned>(g.grid)), block(g.threads);
+    if (g.wide)
+        launch_pdl(k_ln_backward<T, VE, P, true>, grid, block, 0, st, a);
+    else
+        launch_pdl(k_ln_backward<T, VE, P, false>, grid, block, 0, st, a);
+}
+template <typename T, int VE>
+void ln_launch_long(const LnGeom &g, const LnArgs &a, cudaStream_t st) {
+    launch_pdl(k_ln_forward_long<T, VE>, dim3(static_cast<unsigned>(g.grid)), dim3(g.threads), 0, st, a);
+}
+template <typename T, int VE>
+void ln_launch_long(const LnGeom &g, const LnGradArgs &a, cudaStream_t st) {
+    launch_pdl(k_ln_backward_long<T, VE>, dim3(static_cast<unsigned>(g.grid)), dim3(g.threads), 0, st, a);
+}
+template <typename T, typename Args>
+void ln_dispatch(const LnGeom &g, bool vec, const Args &a, cudaStream_t st) {
+    constexpr int E = 16 / static_cast<int>(sizeof(T));
+    if (g.is_long)
+        vec ? ln_launch_long<T, E>(g, a, st) : ln_launch_long<T, 1>(g, a, st);
+    else if (g.P == 8)
+        vec ? ln_launch<T, E, 8>(g, a, st) : ln_launch<T, 1, 8>(g, a, st);
+    else
+        vec ? ln_launch<T, E, 16>(g, a, st) : ln_launch<T, 1, 16>(g, a, st);
+}
+
+// ---- the additive joiner's layer norm ----
+struct JnGeom {
+    int P, threads;
+    int tspan, uspan, tblocks, ublocks;
+    int64_t blocks;
+    size_t smem;
+};
+bool jn_cover(int64_t H, JnGeom *g) {
+    g->P = H <= 4 * JN_MAX_THREADS ? 4 : H <= 8 * JN_MAX_THREADS ? 8 : 32;
+    if (H < 1 || H > 32 * JN_MAX_THREADS) return false;
+    g->threads = static_cast<int>(ceil_div(H, 32 * g->P)) * 32;
+    return true;
+}
+void jn_split(int64_t N, int64_t T, int64_t U1, int64_t tspan, int64_t uspan, JnGeom *g) {
+    g->ublocks = static_cast<int>(ceil_div(U1, uspan));
+    g->uspan = static_cast<int>(ceil_div(U1, g->ublocks));
+    g->ublocks = static_cast<int>(ceil_div(U1, g->uspan));
+    g->tspan = static_cast<int>(tspan);
+    g->tblocks = static_cast<int>(ceil_div(T, tspan));
+    g->blocks = N * g->tblocks * g->ublocks;
+}
+bool jn_forward_geom(int64_t N, int64_t T, int64_t U1, int64_t H, JnGeom *g) {
+    if (!jn_cover(H, g)) return false;
+    const int TF = 32 / g->P;
+    int64_t uspan = U1 < 32 ? U1 : 32;
+    while (uspan > 1 && N * ceil_div(T, TF) * ceil_div(U1, uspan) < 2 * kSms) uspan = (uspan + 1) / 2;
+    jn_split(N, T, U1, TF, uspan, g);
+    g->smem = 0;
+    return g->blocks <= kMaxGrid - 64;
+}
+bool jn_grad_geom(int64_t N, int64_t T, int64_t U1, int64_t H, JnGeom *g) {
+    if (!jn_cover(H, g)) return false;
+    const int TF = 32 / g->P;
+    const int64_t per_context = static_cast<int64_t>(g->threads) * g->P * 4;
+    int64_t uspan = (48 * 1024) / per_context;
+    uspan = uspan < 1 ? 1 : uspan > U1 ? U1 : uspan;
+    int64_t tspan = 8 * TF;
+    while (tspan > TF && N * ceil_div(T, tspan) * ceil_div(U1, uspan) < 8 * kSms) tspan /= 2;
+    while (uspan > 1 && N * ceil_div(T, tspan) * ceil_div(U1, uspan) < kSms) uspan = (uspan + 1) / 2;
+    jn_split(N, T, U1, tspan, uspan, g);
+    g->smem = static_cast<size_t>(g->uspan) * per_context;
+    return g->blocks <= kMaxGrid;
+}
+bool jn_dims_ok(int64_t N, int64_t T, int64_t U1, int64_t H) {
+    return N >= 0 && N <= 65535 && T >= 0 && U1 >= 1 && H >= 1 && H < (int64_t(1) << 31) && T * U1 < (int64_t(1) << 31) &&
+           N * T * U1 < (int64_t(1) << 38);
+}
+struct JnSaved {
+    size_t cu, fm, gm, rstd, total;
+};
+JnSaved jn_saved(int64_t N, int64_t T, int64_t U1, int64_t packed_rows, int want_grad) {
+    JnSaved s;
+    size_t o = 0;
+    s.cu = o;
+    if (packed_rows >= 0) o = align256(o + static_cast<size_t>(N + 1) * 8);
+    s.fm = s.gm = s.rstd = o;
+    if (want_grad) {
+        s.gm = align256(s.fm + static_cast<size_t>(N * T) * 4);
+        s.rstd = align256(s.gm + static_cast<size_t>(N * U1) * 4);
+        o = align256(s.rstd + static_cast<size_t>(packed_rows >= 0 ? packed_rows : N * T * U1) * 4);
+    }
+    s.total = o;
+    return s;
+}
+struct JnWs {
+    size_t f, g, w, total;
+};
+JnWs jn_ws(int64_t N, int64_t T, int64_t U1, int64_t H, const JnGeom &g) {
+    JnWs w;
+    w.f = 0;
+    w.g = align256(static_cast<size_t>(N) * g.ublocks * T * H * 4);
+    w.w = align256(w.g + static_cast<size_t>(N) * g.tblocks * U1 * H * 4);
+    w.total = align256(w.w + 2 * static_cast<size_t>(g.blocks) * H * 4);
+    return w;
+}
+JnShape jn_shape(const int32_t *lx, const int32_t *ly, const int64_t *cu, int64_t packed_rows, int64_t N, int64_t T, int64_t U1,
+                 int64_t H, const JnGeom &g) {
+    JnShape s;
+    s.lx = lx;
+    s.ly = ly;
+    s.cu = cu;
+    s.packed_rows = packed_rows;
+    s.N = static_cast<int>(N);
+    s.T = static_cast<int>(T);
+    s.U1 = static_cast<int>(U1);
+    s.H = static_cast<int>(H);
+    s.tspan = g.tspan;
+    s.uspan = g.uspan;
+    s.tblocks = g.tblocks;
+    s.ublocks = g.ublocks;
+    return s;
+}
+template <typename T, int P>
+void jn_launch(const JnGeom &g, bool vec, const JnArgs &a, unsigned grid, cudaStream_t st) {
+    if (vec)
+        launch_pdl(k_joint_norm<T, 4, P, 32 / P>, dim3(grid), dim3(g.threads), 0, st, a);
+    else
+        launch_pdl(k_joint_norm<T, 1, P, 32 / P>, dim3(grid), dim3(g.threads), 0, st, a);
+}
+template <typename Args>
+int jn_launch_grad(void (*kernel)(Args), const JnGeom &g, const Args &a, cudaStream_t st) {
+    // 48 KB with the kernel's static 4 KB need no attribute; it belongs to the current device: set with the launch
+    if (g.smem > 44 * 1024 &&
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(g.smem)) != cudaSuccess)
+        return check_launch("joint_norm_grad smem attribute");
+    launch_pdl(kernel, dim3(static_cast<unsigned>(g.blocks)), dim3(g.threads), g.smem, st, a);
+    return check_launch("joint_norm_grad");
+}
+
+// ---- adjustment of logits ----
+// Frames of a block: enough blocks for a few waves, and as many frames as that leaves, since the set-up of a
+// block (histories, bias, mask) is paid once for all its frames.
+struct AdjGeom {
+    int64_t tspan, chunks;
+};
+AdjGeom adj_geom(int64_t N, int64_t T, int64_t U1, int64_t V) {
+    AdjGeom g;
+    const int64_t tiles = ceil_div(U1 * V, 1024);
+    g.tspan = 64;
+    while (g.tspan > ADJ_UNROLL && N * tiles * ceil_div(T, g.tspan) < 16 * kSms) g.tspan /= 2;
+    g.chunks = T > 0 ? ceil_div(T, g.tspan) : 1;
+    return g;
+}
+bool adj_dims_ok(int64_t N, int64_t T, int64_t U1, int64_t V) {
+    return N >= 0 && N <= kMaxGrid && T >= 0 && U1 >= 1 && V >= 1 && U1 < (int64_t(1) << 31) && V < (int64_t(1) << 31) &&
+           T < (int64_t(1) << 31) && U1 * V < (int64_t(1) << 31) - 4096;
+}
+template <typename T, int VE, bool GRAD>
+int adj_launch(AdjArgs &a, int64_t N, bool tail, cudaStream_t st) {
+    const int64_t plane = static_cast<int64_t>(a.U1) * a.V;
+    const int64_t chunks_of_plane = ceil_div(plane, VE);
+    const int threads = chunks_of_plane < ADJ_THREADS ? static_cast<int>(ceil_div(chunks_of_plane, 32) * 32) : ADJ_THREADS;
+    a.tiles = static_cast<int>(ceil_div(chunks_of_plane, threads));
+    const int64_t blocks = N * a.tiles * a.chunks;
+    if (blocks > kMaxGrid - 64) return CTCT_ERR_UNSUPPORTED;
+    a.main_blocks = static_cast<unsigned>(blocks);
+    launch_pdl(k_adjust<T, VE, GRAD>, dim3(static_cast<unsigned>(blocks + (tail ? 16 : 0))), dim3(threads), 0, st, a);
+    return check_launch("adjust");
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t ctct_b200_layer_norm_workspace_bytes(int64_t rows, int64_t H, int dtype) {
+    if (rows < 0 || H < 1 || H >= (int64_t(1) << 31) || !dtype_ok(dtype)) return 0;
+    return align256(2 * static_cast<size_t>(ln_geom(rows, H, dtype).grid) * H * 4);
+}
+
+int ctct_b200_layer_norm_forward(const void *x, int64_t x_stride, int dtype, int64_t rows, int64_t H, const void *weight,
+                                 const void *bias, int param_f32, float eps, void *y, float *stats, void *stream) {
+    if (rows < 0 || H < 1 || H >= (int64_t(1) << 31) || !dtype_ok(dtype) || (rows > 0 && (!x || !y))) return CTCT_ERR_ARG;
+    if (rows == 0) return CTCT_OK;
+    const size_t es = esize(dtype);
+    const int64_t E = 16 / static_cast<int64_t>(es);
+    const bool vec = H % E == 0 && x_stride % E == 0 && aligned(x, 16) && aligned(y, 16) && aligned(weight, 16) &&
+                     aligned(bias, 16);
+    LnArgs a{x, x_stride, weight, bias, param_f32 || dtype == CTCT_F32, eps, y, reinterpret_cast<float2 *>(stats), rows,
+             static_cast<int>(H)};
+    const LnGeom g = ln_geom(rows, H, dtype);
+    return with_type(dtype, [&](auto t) {
+        ln_dispatch<decltype(t)>(g, vec, a, static_cast<cudaStream_t>(stream));
+        return check_launch("layer_norm");
+    });
+}
+
+int ctct_b200_layer_norm_backward(const void *dy, int64_t dy_stride, const void *x, int64_t x_stride, int dtype, int64_t rows,
+                                  int64_t H, const void *weight, int param_f32, const float *stats, void *dx, void *dweight,
+                                  void *dbias, void *workspace, size_t workspace_bytes, void *stream) {
+    if (rows < 0 || H < 1 || H >= (int64_t(1) << 31) || !dtype_ok(dtype) || (rows > 0 && (!dy || !x || !stats))) return CTCT_ERR_ARG;
+    const bool params = dweight || dbias;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    LnGeom g = ln_geom(rows, H, dtype);
+    if (params && rows > 0 && (!workspace || !aligned(workspace, 256) || workspace_bytes < 2 * static_cast<size_t>(g.grid) * H * 4))
+        return CTCT_ERR_WORKSPACE;
+    const size_t es = esize(dtype);
+    const int64_t E = 16 / static_cast<int64_t>(es);
+    const bool vec = H % E == 0 && x_stride % E == 0 && dy_stride % E == 0 && aligned(x, 16) && aligned(dy, 16) && aligned(dx, 16) &&
+                     aligned(weight, 16);
+    const int p_f32 = param_f32 || dtype == CTCT_F32;
+    LnGradArgs a{dy, dy_stride, x, x_stride, weight, p_f32, reinterpret_cast<const float2 *>(stats), dx,
+                 params ? static_cast<float *>(workspace) : nullptr, rows, static_cast<int>(H)};
+    return with_type(dtype, [&](auto t) -> int {
+        using T = decltype(t);
+        if (rows > 0) {
+            ln_dispatch<T>(g, vec, a, st);
+            if (int rc = check_launch("layer_norm_grad")) return rc;
+        }
+        if (!params) return CTCT_OK;
+        launch_pdl(k_ln_reduce<T>, dim3(static_cast<unsigned>(ceil_div(H, 32)), 2), dim3(1024), 0, st,
+                   static_cast<const float *>(workspace), rows > 0 ? g.grid : int64_t(0), static_cast<int>(H), dweight, dbias, p_f32);
+        return check_launch("layer_norm_reduce");
+    });
+}
+
+size_t ctct_b200_joint_norm_saved_bytes(int64_t N, int64_t T, int64_t U1, int64_t packed_rows, int want_grad) {
+    if (!jn_dims_ok(N, T, U1, 1)) return 0;
+    return jn_saved(N, T, U1, packed_rows, want_grad).total;
+}
+
+size_t ctct_b200_joint_norm_workspace_bytes(int64_t N, int64_t T, int64_t U1, int64_t H) {
+    JnGeom g;
+    if (!jn_dims_ok(N, T, U1, H) || !jn_grad_geom(N, T, U1, H, &g)) return 0;
+    return jn_ws(N, T, U1, H, g).total;
+}
+
+int ctct_b200_joint_norm_forward(const void *f, int64_t f_sn, int64_t f_st, const void *g, int64_t g_sn, int64_t g_su, int dtype,
+                                 const int32_t *lx, const int32_t *ly, int64_t N, int64_t T, int64_t U1, int64_t H,
+                                 int64_t packed_rows, const void *weight, const void *bias, int param_f32, float eps, void *y,
+                                 int want_grad, void *saved, size_t saved_bytes, void *stream) {
+    const bool packed = packed_rows >= 0;
+    const int64_t rows = packed ? packed_rows : N * T * U1;
+    if (!jn_dims_ok(N, T, U1, H) || !dtype_ok(dtype)) return CTCT_ERR_ARG;
+    if (packed && (!lx || !ly) && N > 0) return CTCT_ERR_ARG;
+    if (rows == 0) return CTCT_OK;
+    if (!y || (N > 0 && T > 0 && (!f || !g))) return CTCT_ERR_ARG;
+    const JnSaved sv = jn_saved(N, T, U1, packed_rows, want_grad);
+    if (sv.total > 0 && (!saved || !aligned(saved, 256) || saved_bytes < sv.total)) return CTCT_ERR_WORKSPACE;
+    JnGeom geo;
+    if (!jn_forward_geom(N, T, U1, H, &geo)) return CTCT_ERR_UNSUPPORTED;
+    char *sb = static_cast<char *>(saved);
+    int64_t *cu = packed ? reinterpret_cast<int64_t *>(sb + sv.cu) : nullptr;
+    if (packed)
+        if (int rc = ctct_b200_packed_offsets(lx, ly, N, T, U1, cu, stream)) return rc;
+    const size_t es = esize(dtype), p_al = (param_f32 || dtype == CTCT_F32) ? 16 : 8;
+    const bool vec = H % 4 == 0 && f_sn % 4 == 0 && f_st % 4 == 0 && g_sn % 4 == 0 && g_su % 4 == 0 && aligned(f, 4 * es) &&
+                     aligned(g, 4 * es) && aligned(y, 4 * es) && aligned(weight, p_al) && aligned(bias, p_al);
+    JnArgs a;
+    a.s = jn_shape(lx, ly, cu, packed_rows, N, T, U1, H, geo);
+    a.f = f;
+    a.g = g;
+    a.f_sn = f_sn;
+    a.f_st = f_st;
+    a.g_sn = g_sn;
+    a.g_su = g_su;
+    a.w = weight;
+    a.b = bias;
+    a.p_f32 = param_f32 || dtype == CTCT_F32;
+    a.eps = eps;
+    a.y = y;
+    a.fm = want_grad ? reinterpret_cast<float *>(sb + sv.fm) : nullptr;
+    a.gm = want_grad ? reinterpret_cast<float *>(sb + sv.gm) : nullptr;
+    a.rstd = want_grad ? reinterpret_cast<float *>(sb + sv.rstd) : nullptr;
+    a.main_blocks = static_cast<unsigned>(geo.blocks);
+    const unsigned grid = static_cast<unsigned>(geo.blocks + (packed ? 16 : 0));
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return with_type(dtype, [&](auto t) {
+        using E = decltype(t);
+        if (geo.P == 4)
+            jn_launch<E, 4>(geo, vec, a, grid, st);
+        else if (geo.P == 8)
+            jn_launch<E, 8>(geo, vec, a, grid, st);
+        else
+            jn_launch<E, 32>(geo, vec, a, grid, st);
+        return check_launch("joint_norm");
+    });
+}
+
+int ctct_b200_joint_norm_backward(const void *dy, const void *f, int64_t f_sn, int64_t f_st, const void *g, int64_t g_sn,
+                                  int64_t g_su, int dtype, const int32_t *lx, const int32_t *ly, int64_t N, int64_t T, int64_t U1,
+                                  int64_t H, int64_t packed_rows, const void *weight, int param_f32, const void *saved,
+                                  size_t saved_bytes, void *df, void *dg, void *dweight, void *dbias, void *workspace,
+                                  size_t workspace_bytes, void *stream) {
+    const bool packed = packed_rows >= 0;
+    const int64_t rows = packed ? packed_rows : N * T * U1;
+    if (!jn_dims_ok(N, T, U1, H) || !dtype_ok(dtype)) return CTCT_ERR_ARG;
+    if (packed && (!lx || !ly) && N > 0) return CTCT_ERR_ARG;
+    JnGeom geo;
+    if (!jn_grad_geom(N, T, U1, H, &geo)) return CTCT_ERR_UNSUPPORTED;
+    const JnSaved sv = jn_saved(N, T, U1, packed_rows, 1);
+    const JnWs ws = jn_ws(N, T, U1, H, geo);
+    if (rows > 0 && (!dy || (N > 0 && T > 0 && (!f || !g)))) return CTCT_ERR_ARG;
+    if (rows > 0 && geo.blocks > 0 && (!saved || !aligned(saved, 256) || saved_bytes < sv.total)) return CTCT_ERR_WORKSPACE;
+    if (geo.blocks > 0 && (!workspace || !aligned(workspace, 256) || workspace_bytes < ws.total)) return CTCT_ERR_WORKSPACE;
+    const char *sb = static_cast<const char *>(saved);
+    char *wb = static_cast<char *>(workspace);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const size_t es = esize(dtype), p_al = (param_f32 || dtype == CTCT_F32) ? 16 : 8;
+    const bool vec = H % 4 == 0 && f_sn % 4 == 0 && f_st % 4 == 0 && g_sn % 4 == 0 && g_su % 4 == 0 && aligned(f, 4 * es) &&
+                     aligned(g, 4 * es) && aligned(dy, 4 * es) && aligned(weight, p_al);
+    JnGradArgs a;
+    a.s = jn_shape(lx, ly, packed && rows > 0 ? reinterpret_cast<const int64_t *>(sb + sv.cu) : nullptr, packed_rows, N, T, U1, H, geo);
+    a.f = f;
+    a.g = g;
+    a.f_sn = f_sn;
+    a.f_st = f_st;
+    a.g_sn = g_sn;
+    a.g_su = g_su;
+    a.w = weight;
+    a.p_f32 = param_f32 || dtype == CTCT_F32;
+    a.dy = dy;
+    a.fm = reinterpret_cast<const float *>(sb + sv.fm);
+    a.gm = reinterpret_cast<const float *>(sb + sv.gm);
+    a.rstd = reinterpret_cast<const float *>(sb + sv.rstd);
+    a.part_f = reinterpret_cast<float *>(wb + ws.f);
+    a.part_g = reinterpret_cast<float *>(wb + ws.g);
+    a.part_w = reinterpret_cast<float *>(wb + ws.w);
+    JnReduceArgs r;
+    r.s = a.s;
+    r.part_f = a.part_f;
+    r.part_g = a.part_g;
+    r.part_w = a.part_w;
+    r.df = df;
+    r.dg = dg;
+    r.dw = dweight;
+    r.db = dbias;
+    r.p_f32 = a.p_f32;
+    const bool some = rows > 0 && geo.blocks > 0;
+    r.parts_w = some ? geo.blocks : 0;
+    r.no_rows = !some;
+    const int64_t wb_n = 2 * ceil_div(H, 32), fb = ceil_div(N * T * H, 1024), gb = ceil_div(N * U1 * H, 1024);
+    if (wb_n + fb + gb > kMaxGrid) return CTCT_ERR_UNSUPPORTED;
+    r.w_blocks = static_cast<unsigned>(wb_n);
+    r.f_blocks = static_cast<unsigned>(fb);
+    return with_type(dtype, [&](auto t) -> int {
+        using E = decltype(t);
+        if (some) {
+            int rc;
+            if (geo.P == 4)
+                rc = jn_launch_grad(vec ? k_joint_norm_grad<E, 4, 4, 8> : k_joint_norm_grad<E, 1, 4, 8>, geo, a, st);
+            else if (geo.P == 8)
+                rc = jn_launch_grad(vec ? k_joint_norm_grad<E, 4, 8, 4> : k_joint_norm_grad<E, 1, 8, 4>, geo, a, st);
+            else
+                rc = jn_launch_grad(vec ? k_joint_norm_grad<E, 4, 32, 1> : k_joint_norm_grad<E, 1, 32, 1>, geo, a, st);
+            if (rc) return rc;
+        }
+        launch_pdl(k_joint_norm_reduce<E>, dim3(static_cast<unsigned>(wb_n + fb + gb)), dim3(1024), 0, st, r);
+        return check_launch("joint_norm_reduce");
+    });
+}
+
+size_t ctct_b200_adjust_workspace_bytes(int64_t N, int64_t T, int64_t U1, int64_t V) {
+    if (!adj_dims_ok(N, T, U1, V)) return 0;
+    return align256(static_cast<size_t>(N) * adj_geom(N, T, U1, V).chunks * U1 * V * 4);
+}
+
+namespace {
+
+struct AdjCall {
+    const int32_t *tokens, *tokens_len;
+    int64_t tokens_pitch;
+    const int32_t *lx, *ly;
+    int64_t N, T, U1, V, packed_rows;
+    const int64_t *cu;
+    const void *bias;
+    int bias_kind, bias_f32;
+    const int32_t *allowed;
+    int mask_kind;
+    float rho, presence, frequency;
+    const float *rho_n, *presence_n, *frequency_n;
+};
+// the common part of both directions; CTCT_OK, or why the call is refused
+int adj_fill(const AdjCall &c, int dtype, AdjArgs *a) {
+    if (!adj_dims_ok(c.N, c.T, c.U1, c.V) || !dtype_ok(dtype)) return CTCT_ERR_ARG;
+    if (c.packed_rows >= 0 && (!c.lx || !c.ly || !c.cu)) return CTCT_ERR_ARG;
+    if (c.bias_kind < 0 || c.bias_kind > 3 || c.mask_kind < 0 || c.mask_kind > 3) return CTCT_ERR_ARG;
+    if ((c.mask_kind != 0) != (c.allowed != nullptr)) return CTCT_ERR_ARG;
+    if (c.tokens_pitch < 0 || (c.tokens && !c.tokens_len && c.tokens_pitch < c.U1 - 1)) return CTCT_ERR_ARG;
+    if (!c.rho_n && !(c.rho > 0.0f)) return CTCT_ERR_ARG;
+    const int64_t words = ceil_div(c.V, 32);
+    a->tokens = c.tokens_pitch > 0 ? c.tokens : nullptr;
+    a->tokens_len = c.tokens_len;
+    a->L = c.tokens_pitch;
+    a->lx = c.lx;
+    a->ly = c.ly;
+    a->cu = c.packed_rows >= 0 ? c.cu : nullptr;
+    a->packed_rows = c.packed_rows;
+    a->bias = c.bias;
+    a->bias_f32 = c.bias_f32 || dtype == CTCT_F32;
+    a->bias_sn = c.bias_kind == 2 ? c.V : c.bias_kind == 3 ? c.U1 * c.V : 0;
+    a->bias_su = c.bias_kind == 3 ? c.V : 0;
+    a->allowed = reinterpret_cast<const unsigned *>(c.allowed);
+    a->mask_sn = c.mask_kind == 2 ? words : c.mask_kind == 3 ? c.U1 * words : 0;
+    a->mask_su = c.mask_kind == 3 ? words : 0;
+    a->rho = c.rho;
+    a->presence = c.presence;
+    a->frequency = c.frequency;
+    a->rho_n = c.rho_n;
+    a->presence_n = c.presence_n;
+    a->frequency_n = c.frequency_n;
+    a->N = static_cast<int>(c.N);
+    a->T = static_cast<int>(c.T);
+    a->U1 = static_cast<int>(c.U1);
+    a->V = static_cast<int>(c.V);
+    const AdjGeom g = adj_geom(c.N, c.T, c.U1, c.V);
+    a->tspan = static_cast<int>(g.tspan);
+    a->chunks = static_cast<int>(g.chunks);
+    return CTCT_OK;
+}
+
+}  // namespace
+
+int ctct_b200_adjust_forward(const void *logits, int64_t row_stride, int dtype, const int32_t *tokens, int64_t tokens_pitch,
+                             const int32_t *tokens_lengths, const int32_t *lx, const int32_t *ly, int64_t N, int64_t T, int64_t U1,
+                             int64_t V, int64_t packed_rows, int64_t *cu_rows, const void *bias, int bias_kind, int bias_f32,
+                             const int32_t *allowed, int mask_kind, float repetition, float presence, float frequency,
+                             const float *repetition_n, const float *presence_n, const float *frequency_n, void *out, void *stream) {
+    AdjArgs a = {};
+    const AdjCall c{tokens, tokens_lengths, tokens_pitch, lx, ly, N, T, U1, V, packed_rows, cu_rows, bias, bias_kind, bias_f32,
+                    allowed, mask_kind, repetition, presence, frequency, repetition_n, presence_n, frequency_n};
+    if (int rc = adj_fill(c, dtype, &a)) return rc;
+    if ((bias_kind != 0) != (bias != nullptr) || row_stride < 0 || (row_stride > 0 && (T != 1 || U1 != 1 || packed_rows >= 0)))
+        return CTCT_ERR_ARG;
+    const int64_t rows = packed_rows >= 0 ? packed_rows : N * T * U1;
+    if (rows == 0) return CTCT_OK;
+    if (!logits || !out) return CTCT_ERR_ARG;
+    if (packed_rows >= 0)
+        if (int rc = ctct_b200_packed_offsets(lx, ly, N, T, U1, cu_rows, stream)) return rc;
+    a.x = logits;
+    a.x_sn = row_stride;
+    a.y = out;
+    const size_t es = esize(dtype);
+    const int64_t E = 16 / static_cast<int64_t>(es);
+    const bool vec = V % E == 0 && row_stride % E == 0 && aligned(logits, 16) && aligned(out, 16) && aligned(bias, 16);
+    return with_type(dtype, [&](auto t) {
+        using T_ = decltype(t);
+        constexpr int VE = 16 / static_cast<int>(sizeof(T_));
+        const cudaStream_t st = static_cast<cudaStream_t>(stream);
+        return vec ? adj_launch<T_, VE, false>(a, N, packed_rows >= 0, st) : adj_launch<T_, 1, false>(a, N, packed_rows >= 0, st);
+    });
+}
+
+int ctct_b200_adjust_backward(const void *dy, const void *logits, int64_t row_stride, int dtype, const int32_t *tokens,
+                              int64_t tokens_pitch, const int32_t *tokens_lengths, const int32_t *lx, const int32_t *ly, int64_t N,
+                              int64_t T, int64_t U1, int64_t V, int64_t packed_rows, const int64_t *cu_rows, int bias_kind,
+                              int bias_f32, const int32_t *allowed, int mask_kind, float repetition, const float *repetition_n,
+                              void *dx, void *dbias, void *workspace, size_t workspace_bytes, void *stream) {
+    AdjArgs a = {};
+    const AdjCall c{tokens, tokens_lengths, tokens_pitch, lx, ly, N, T, U1, V, packed_rows, cu_rows, nullptr, bias_kind, bias_f32,
+                    allowed, mask_kind, repetition, 0.0f, 0.0f, repetition_n, nullptr, nullptr};
+    if (int rc = adj_fill(c, dtype, &a)) return rc;
+    if ((dbias && bias_kind == 0) || row_stride < 0 || (row_stride > 0 && (T != 1 || U1 != 1 || packed_rows >= 0))) return CTCT_ERR_ARG;
+    const int64_t rows = packed_rows >= 0 ? packed_rows : N * T * U1;
+    const size_t need = static_cast<size_t>(N) * a.chunks * U1 * V * 4;
+    if (rows > 0 && (!dy || (dx && a.tokens && (repetition_n || repetition != 1.0f) && !logits))) return CTCT_ERR_ARG;
+    if (rows > 0 && dbias && (!workspace || !aligned(workspace, 256) || workspace_bytes < need)) return CTCT_ERR_WORKSPACE;
+    a.x = logits;
+    a.x_sn = row_stride;
+    a.dy = dy;
+    a.y = dx;
+    a.part = dbias ? static_cast<float *>(workspace) : nullptr;
+    const size_t es = esize(dtype);
+    const int64_t E = 16 / static_cast<int64_t>(es);
+    const bool vec = V % E == 0 && row_stride % E == 0 && aligned(logits, 16) && aligned(dx, 16) && aligned(dy, 16);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return with_type(dtype, [&](auto t) -> int {
+        using T_ = decltype(t);
+        constexpr int VE = 16 / static_cast<int>(sizeof(T_));
+        if (rows > 0 && N * T > 0) {
+            const bool tail = packed_rows >= 0 && dx;
+            const int rc = vec ? adj_launch<T_, VE, true>(a, N, tail, st) : adj_launch<T_, 1, true>(a, N, tail, st);
+            if (rc) return rc;
+        }
+        if (!dbias) return CTCT_OK;
+        const int64_t P = rows > 0 && N * T > 0 ? a.chunks : 0;  // no row: zeros
+        ReduceArgs r{static_cast<const float *>(workspace), dbias, a.bias_f32, 0, 0};
+        int64_t outer = 1;
+        if (bias_kind == 1) {
+            r.P = N * P * U1;
+            r.C = V;
+        } else if (bias_kind == 2) {
+            outer = N;
+            r.P = P * U1;
+            r.C = V;
+        } else {
+            outer = N;
+            r.P = P;
+            r.C = U1 * V;
+        }
+        if (outer == 0) return CTCT_OK;
+        const int64_t col_blocks = ceil_div(r.C, 32);
+        if (outer * col_blocks > kMaxGrid) return CTCT_ERR_UNSUPPORTED;
+        launch_pdl(k_adjust_reduce<T_>, dim3(static_cast<unsigned>(outer * col_blocks)), dim3(1024), 0, st, r);
+        return check_launch("adjust_reduce");
+    });
+}
+
+}  // extern "C"
