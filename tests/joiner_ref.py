@@ -19,7 +19,7 @@ def half_step(v, dtype):
     return v.abs() * (torch.finfo(dtype).eps / 2) + tiny
 
 
-def norm_reference(s, w, b, eps, dy, amax, k, rows_k, dtype, pdtype):
+def norm_reference(s, w, b, eps, dy, amax, k, rows_k, dtype, pdtype, parts=None):
     """Layer norm of the rows `s` (R, H) float64 with gradients for `dy` (or None), and bounds of everything.
 
     amax: (R, 1) largest magnitude that entered a row's float32 sums; k: longest chain of additions along a row,
@@ -48,8 +48,11 @@ def norm_reference(s, w, b, eps, dy, amax, k, rows_k, dtype, pdtype):
     e_ds = e_ds + 3 * Er * r * (q.abs() + c1.abs() + (xh * c2).abs())
     dw, db = (dy * xh).sum(0), dy.sum(0)
     val.update(ds=ds, dw=dw, db=db)
+    # a sum of ds over rows may be taken as three sums, of r q, r c1 and r xh c2: its rounding goes by their magnitudes
+    val["terms"] = r * (q.abs() + c1.abs() + (xh * c2).abs())
     tol["ds"] = e_ds
-    tol["dw"] = (dy.abs() * E).sum(0) + (rows_k + 4) * U * (dy * xh).abs().sum(0) + half_step(dw, pdtype)
+    # dy xh may be summed as dy f r and dy g r apart (f, g centred, at most amax): "parts" is the bound of |f| + |g|
+    tol["dw"] = (dy.abs() * E).sum(0) + (rows_k + 4) * U * (dy.abs() * (xh.abs() if parts is None else parts * r)).sum(0) + half_step(dw, pdtype)
     tol["db"] = (rows_k + 4) * U * dy.abs().sum(0) + half_step(db, pdtype)
     return val, tol
 

@@ -81,15 +81,17 @@ def test_training_step(W):
         dx = torch.where(per_row(ok), dzv * torch.where(hit, torch.where(x > 0, 1 / 1.2, 1.2), 1.0), 0.0)
         dh, e_h = dx @ d["out"].T, (V + 8) * U * (dx.abs() @ d["out"].abs().T)   # V products in float32
         amax = (p["f"].abs().amax(-1).unsqueeze(2) + p["g"].abs().amax(-1).unsqueeze(1))[valid].unsqueeze(-1).double()
-        val, tol = norm_reference(s, p["w"], p["b"], 1e-5, dh, amax, 80, s.size(0) + 64, torch.float32, torch.float32)
+        mag = lambda t: (t.double() - t.double().mean(-1, keepdim=True)).abs()  # noqa: E731
+        parts = (mag(p["f"]).unsqueeze(2) + mag(p["g"]).unsqueeze(1))[valid]
+        val, tol = norm_reference(s, p["w"], p["b"], 1e-5, dh, amax, 80, s.size(0) + 64, torch.float32, torch.float32, parts)
         r = (sn.square().mean(-1, keepdim=True) + 1e-5).rsqrt()
         xh, we = (sn * r).abs(), d["w"].abs() * e_h
         e_ds = tol["ds"] + r * (we + we.mean(-1, keepdim=True) + xh * (we * xh).mean(-1, keepdim=True))
         full = torch.zeros((N, T, U1, H), device=DEV, dtype=torch.float64)
-        ds, e = full.clone(), full.clone()
-        ds[valid], e[valid] = val["ds"], e_ds
-        check("df", got["f"], ds.sum(2), e.sum(2) + 80 * U * ds.abs().sum(2))
-        check("dg", got["g"], ds.sum(1), e.sum(1) + 80 * U * ds.abs().sum(1))
+        ds, e, terms = full.clone(), full.clone(), full.clone()
+        ds[valid], e[valid], terms[valid] = val["ds"], e_ds, val["terms"]
+        check("df", got["f"], ds.sum(2), e.sum(2) + 80 * U * terms.sum(2))
+        check("dg", got["g"], ds.sum(1), e.sum(1) + 80 * U * terms.sum(1))
         check("dw", got["w"], val["dw"], tol["dw"] + (e_h * xh).sum(0))
         check("db", got["b"], val["db"], tol["db"] + e_h.sum(0))
         want = torch.where(per_row(ok), dzv, 0.0).sum(0)

@@ -168,14 +168,16 @@ def _check_joint(W, f, g, lx, ly, w, b, eps, dy, packed):
     s = (f.double().unsqueeze(2) + g.double().unsqueeze(1))[valid]
     amax = (f.double().abs().amax(-1).unsqueeze(2) + g.double().abs().amax(-1).unsqueeze(1))[valid].unsqueeze(-1)
     # dw and db: chains of at most 64 frames x 128 contexts in a block, then the blocks
-    val, tol = norm_reference(s, w, b, eps, dy[valid], amax, _chain(H), min(s.size(0), 64 * 128) + 64, f.dtype, w.dtype)
+    mag = lambda t: (t.double() - t.double().mean(-1, keepdim=True)).abs()  # noqa: E731
+    parts = (mag(f).unsqueeze(2) + mag(g).unsqueeze(1))[valid]
+    val, tol = norm_reference(s, w, b, eps, dy[valid], amax, _chain(H), min(s.size(0), 64 * 128) + 64, f.dtype, w.dtype, parts)
     check("y", rows, val["y"], tol["y"])
     full = torch.zeros((N, T, U1, H), dtype=torch.float64, device=DEV)
-    ds, e = full.clone(), full.clone()
-    ds[valid], e[valid] = val["ds"], tol["ds"]
+    ds, e, terms = full.clone(), full.clone(), full.clone()
+    ds[valid], e[valid], terms[valid] = val["ds"], tol["ds"], val["terms"]
     for name, t, dim, n in (("df", got[0], 2, U1), ("dg", got[1], 1, T)):
         want = ds.sum(dim)
-        check(name, t, want, e.sum(dim) + (n + 8) * U * ds.abs().sum(dim) + half_step(want, f.dtype))
+        check(name, t, want, e.sum(dim) + (n + 8) * U * terms.sum(dim) + half_step(want, f.dtype))
     check("dw", got[2], val["dw"], tol["dw"])
     check("db", got[3], val["db"], tol["db"])
     return got

@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(1024) k_adjust_reduce(const ReduceArgs a) {
     __shared__ float sm[32][33];
     pdl_wait();
     const unsigned col_blocks = static_cast<unsigned>((a.C + 31) / 32);
-    reduce_columns<T>(a, blockIdx.x % col_blocks, blockIdx.x / col_blocks, sm);
+    reduce_columns<T, 32, 32>(a, blockIdx.x % col_blocks, blockIdx.x / col_blocks, sm);
 }
 
 }  // namespace ctct

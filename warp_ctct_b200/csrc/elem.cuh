@@ -103,6 +103,51 @@ __device__ __forceinline__ void load_param(const void *p, int is_f32, int64_t at
     }
 }
 
+// Two float32 in one 64-bit register, added and multiplied by one instruction (sm_100): the kernels that are held
+// back by instruction issue do their arithmetic in pairs.
+struct F2 {
+    unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float x, float y) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void split(const F2 &a, float &x, float &y) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a.v));
+}
+__device__ __forceinline__ F2 add2(const F2 &a, const F2 &b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 mul2(const F2 &a, const F2 &b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 fma2(const F2 &a, const F2 &b, const F2 &c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+__device__ __forceinline__ float sum2(const F2 &a) {
+    float x, y;
+    split(a, x, y);
+    return x + y;
+}
+// P values as P / 2 pairs and back
+template <int P>
+__device__ __forceinline__ void pair_up(const float (&x)[P], F2 (&y)[P / 2]) {
+#pragma unroll
+    for (int i = 0; i < P / 2; ++i) y[i] = f2(x[2 * i], x[2 * i + 1]);
+}
+template <int P>
+__device__ __forceinline__ void unpair(const F2 (&y)[P / 2], float (&x)[P]) {
+#pragma unroll
+    for (int i = 0; i < P / 2; ++i) split(y[i], x[2 * i], x[2 * i + 1]);
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -127,35 +172,37 @@ __device__ __forceinline__ void block_sum(float (&v)[K], float *sm, int slot) {
 }
 
 // out[o][c] = sum over p of part[o][p][c]: the partial sums that the blocks of a launch leave, added
-// in a fixed order, so that gradients do not depend on which block came first.  Blocks of 32 columns x 32
-// threads; a thread adds every 32nd partial, shared memory joins the 32.
+// in a fixed order, so that gradients do not depend on which block came first.  Blocks of COLS columns x LANES
+// threads; a thread adds every LANES-th partial, shared memory joins them.
 struct ReduceArgs {
     const float *part;
     void *out;
     int out_f32;     // out in float32, else in T
     int64_t P, C;    // partials, columns
 };
-template <typename T>
-__device__ __forceinline__ void reduce_columns(const ReduceArgs &a, int64_t col_block, int64_t o, float (*sm)[33]) {
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const int64_t c = col_block * 32 + tx;
+template <typename T, int COLS, int LANES>
+__device__ __forceinline__ void reduce_columns(const ReduceArgs &a, int64_t col_block, int64_t o, float (*sm)[COLS + 1]) {
+    const int tx = threadIdx.x % COLS, ty = threadIdx.x / COLS;
+    const int64_t c = col_block * COLS + tx;
     float s = 0.0f;
     if (c < a.C) {
         const float *p = a.part + o * a.P * a.C + c;
-        float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        int64_t i = ty;
-        for (; i + 96 < a.P; i += 128)
+        float s8[8];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) s4[k] += p[(i + 32 * k) * a.C];
-        for (; i < a.P; i += 32) s4[0] += p[i * a.C];
-        s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+        for (int k = 0; k < 8; ++k) s8[k] = 0.0f;
+        int64_t i = ty;
+        for (; i + 7 * LANES < a.P; i += 8 * LANES)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s8[k] += p[(i + LANES * k) * a.C];
+        for (; i < a.P; i += LANES) s8[0] += p[i * a.C];
+        s = ((s8[0] + s8[1]) + (s8[2] + s8[3])) + ((s8[4] + s8[5]) + (s8[6] + s8[7]));
     }
     sm[ty][tx] = s;
     __syncthreads();
     if (ty == 0 && c < a.C) {
         float t = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 32; ++k) t += sm[k][tx];
+        for (int k = 0; k < LANES; ++k) t += sm[k][tx];
         if (a.out_f32)
             static_cast<float *>(a.out)[o * a.C + c] = t;
         else

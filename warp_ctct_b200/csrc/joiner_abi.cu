@@ -92,17 +92,14 @@ void ln_dispatch(const LnGeom &g, bool vec, const Args &a, cudaStream_t st) {
 
 // ---- the additive joiner's layer norm ----
 struct JnGeom {
-    int P, threads;
+    int P, threads, slices;
     int tspan, uspan, tblocks, ublocks;
     int64_t blocks;
     size_t smem;
 };
-bool jn_cover(int64_t H, JnGeom *g) {
-    g->P = H <= 4 * JN_MAX_THREADS ? 4 : H <= 8 * JN_MAX_THREADS ? 8 : 32;
-    if (H < 1 || H > 32 * JN_MAX_THREADS) return false;
-    g->threads = static_cast<int>(ceil_div(H, 32 * g->P)) * 32;
-    return true;
-}
+// Forward: columns per thread and frames per block: 8 x 4 up to 2048 columns (16-byte accesses of 16-bit types, at
+// most 256 threads), 32 x 1 beyond, where a row's sums need all threads of a block (a path for completeness).
+constexpr int JN_THREADS = 256, JN_WIDE_THREADS = 512;
 void jn_split(int64_t N, int64_t T, int64_t U1, int64_t tspan, int64_t uspan, JnGeom *g) {
     g->ublocks = static_cast<int>(ceil_div(U1, uspan));
     g->uspan = static_cast<int>(ceil_div(U1, g->ublocks));
@@ -112,26 +109,33 @@ void jn_split(int64_t N, int64_t T, int64_t U1, int64_t tspan, int64_t uspan, Jn
     g->blocks = N * g->tblocks * g->ublocks;
 }
 bool jn_forward_geom(int64_t N, int64_t T, int64_t U1, int64_t H, JnGeom *g) {
-    if (!jn_cover(H, g)) return false;
+    if (H < 1 || H > 32 * JN_WIDE_THREADS) return false;
+    g->P = H <= 8 * JN_THREADS ? 8 : 32;
+    g->threads = static_cast<int>(ceil_div(H, 32 * g->P)) * 32;
     const int TF = 32 / g->P;
     int64_t uspan = U1 < 32 ? U1 : 32;
     while (uspan > 1 && N * ceil_div(T, TF) * ceil_div(U1, uspan) < 2 * kSms) uspan = (uspan + 1) / 2;
     jn_split(N, T, U1, TF, uspan, g);
-    g->smem = 0;
     return g->blocks <= kMaxGrid - 64;
 }
+// Backward: threads are independent, so a block has the columns that 256 threads cover and further blocks the
+// rest.  A block's contexts are as many as its accumulators' share of shared memory holds; its frames as
+// many as leave enough blocks.
 bool jn_grad_geom(int64_t N, int64_t T, int64_t U1, int64_t H, JnGeom *g) {
-    if (!jn_cover(H, g)) return false;
-    const int TF = 32 / g->P;
-    const int64_t per_context = static_cast<int64_t>(g->threads) * g->P * 4;
-    int64_t uspan = (48 * 1024) / per_context;
+    if (H < 1 || H > 32 * JN_WIDE_THREADS) return false;
+    const int64_t all = ceil_div(H, 32 * JG_P) * 32;
+    g->P = JG_P;
+    g->threads = static_cast<int>(all < JG_MAX_THREADS ? all : JG_MAX_THREADS);
+    g->slices = static_cast<int>(ceil_div(H, JG_P * JG_MAX_THREADS));
+    const int64_t per_context = static_cast<int64_t>(g->threads) * JG_P * 4;
+    int64_t uspan = (32 * 1024) / per_context;
     uspan = uspan < 1 ? 1 : uspan > U1 ? U1 : uspan;
-    int64_t tspan = 8 * TF;
-    while (tspan > TF && N * ceil_div(T, tspan) * ceil_div(U1, uspan) < 8 * kSms) tspan /= 2;
+    int64_t tspan = 16 * JG_TF;
+    while (tspan > JG_TF && N * ceil_div(T, tspan) * ceil_div(U1, uspan) < 16 * kSms) tspan /= 2;
     while (uspan > 1 && N * ceil_div(T, tspan) * ceil_div(U1, uspan) < kSms) uspan = (uspan + 1) / 2;
     jn_split(N, T, U1, tspan, uspan, g);
     g->smem = static_cast<size_t>(g->uspan) * per_context;
-    return g->blocks <= kMaxGrid;
+    return g->blocks * g->slices <= kMaxGrid;
 }
 bool jn_dims_ok(int64_t N, int64_t T, int64_t U1, int64_t H) {
     return N >= 0 && N <= 65535 && T >= 0 && U1 >= 1 && H >= 1 && H < (int64_t(1) << 31) && T * U1 < (int64_t(1) << 31) &&
@@ -155,14 +159,15 @@ JnSaved jn_saved(int64_t N, int64_t T, int64_t U1, int64_t packed_rows, int want
     return s;
 }
 struct JnWs {
-    size_t f, g, w, total;
+    size_t a, b, w, c, total;
 };
-JnWs jn_ws(int64_t N, int64_t T, int64_t U1, int64_t H, const JnGeom &g) {
+JnWs jn_ws(int64_t N, int64_t T, int64_t U1, int64_t H, int64_t rows, const JnGeom &g) {
     JnWs w;
-    w.f = 0;
-    w.g = align256(static_cast<size_t>(N) * g.ublocks * T * H * 4);
-    w.w = align256(w.g + static_cast<size_t>(N) * g.tblocks * U1 * H * 4);
-    w.total = align256(w.w + 2 * static_cast<size_t>(g.blocks) * H * 4);
+    w.a = 0;
+    w.b = align256(static_cast<size_t>(N) * g.ublocks * T * H * 4);
+    w.w = align256(w.b + static_cast<size_t>(N) * g.tblocks * U1 * H * 4);
+    w.c = align256(w.w + 2 * static_cast<size_t>(g.blocks) * H * 4);
+    w.total = align256(w.c + static_cast<size_t>(g.slices * (g.threads / 32)) * rows * 8);
     return w;
 }
 JnShape jn_shape(const int32_t *lx, const int32_t *ly, const int64_t *cu, int64_t packed_rows, int64_t N, int64_t T, int64_t U1,
@@ -182,23 +187,15 @@ JnShape jn_shape(const int32_t *lx, const int32_t *ly, const int64_t *cu, int64_
     s.ublocks = g.ublocks;
     return s;
 }
-template <typename T, int P>
+template <typename T>
 void jn_launch(const JnGeom &g, bool vec, const JnArgs &a, unsigned grid, cudaStream_t st) {
-    if (vec)
-        launch_pdl(k_joint_norm<T, 4, P, 32 / P>, dim3(grid), dim3(g.threads), 0, st, a);
+    constexpr int VE = 16 / static_cast<int>(sizeof(T));
+    if (g.P == 8)
+        launch_pdl(vec ? k_joint_norm<T, VE, 8, 4> : k_joint_norm<T, 1, 8, 4>, dim3(grid), dim3(g.threads), 0, st, a);
     else
-        launch_pdl(k_joint_norm<T, 1, P, 32 / P>, dim3(grid), dim3(g.threads), 0, st, a);
+        launch_pdl(vec ? k_joint_norm<T, VE, 32, 1> : k_joint_norm<T, 1, 32, 1>, dim3(grid),
+                   dim3(g.threads), 0, st, a);
 }
-template <typename Args>
-int jn_launch_grad(void (*kernel)(Args), const JnGeom &g, const Args &a, cudaStream_t st) {
-    // 48 KB with the kernel's static 4 KB need no attribute; it belongs to the current device: set with the launch
-    if (g.smem > 44 * 1024 &&
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(g.smem)) != cudaSuccess)
-        return check_launch("joint_norm_grad smem attribute");
-    launch_pdl(kernel, dim3(static_cast<unsigned>(g.blocks)), dim3(g.threads), g.smem, st, a);
-    return check_launch("joint_norm_grad");
-}
-
 // ---- adjustment of logits ----
 // Frames of a block: enough blocks for a few waves, and as many frames as that leaves, since the set-up of a
 // block (histories, bias, mask) is paid once for all its frames.
@@ -290,10 +287,10 @@ size_t ctct_b200_joint_norm_saved_bytes(int64_t N, int64_t T, int64_t U1, int64_
     return jn_saved(N, T, U1, packed_rows, want_grad).total;
 }
 
-size_t ctct_b200_joint_norm_workspace_bytes(int64_t N, int64_t T, int64_t U1, int64_t H) {
+size_t ctct_b200_joint_norm_workspace_bytes(int64_t N, int64_t T, int64_t U1, int64_t H, int64_t packed_rows) {
     JnGeom g;
     if (!jn_dims_ok(N, T, U1, H) || !jn_grad_geom(N, T, U1, H, &g)) return 0;
-    return jn_ws(N, T, U1, H, g).total;
+    return jn_ws(N, T, U1, H, packed_rows >= 0 ? packed_rows : N * T * U1, g).total;
 }
 
 int ctct_b200_joint_norm_forward(const void *f, int64_t f_sn, int64_t f_st, const void *g, int64_t g_sn, int64_t g_su, int dtype,
@@ -314,9 +311,9 @@ int ctct_b200_joint_norm_forward(const void *f, int64_t f_sn, int64_t f_st, cons
     int64_t *cu = packed ? reinterpret_cast<int64_t *>(sb + sv.cu) : nullptr;
     if (packed)
         if (int rc = ctct_b200_packed_offsets(lx, ly, N, T, U1, cu, stream)) return rc;
-    const size_t es = esize(dtype), p_al = (param_f32 || dtype == CTCT_F32) ? 16 : 8;
-    const bool vec = H % 4 == 0 && f_sn % 4 == 0 && f_st % 4 == 0 && g_sn % 4 == 0 && g_su % 4 == 0 && aligned(f, 4 * es) &&
-                     aligned(g, 4 * es) && aligned(y, 4 * es) && aligned(weight, p_al) && aligned(bias, p_al);
+    const int64_t E = 16 / static_cast<int64_t>(esize(dtype));
+    const bool vec = H % E == 0 && f_sn % E == 0 && f_st % E == 0 && g_sn % E == 0 && g_su % E == 0 && aligned(f, 16) && aligned(g, 16) &&
+                     aligned(y, 16) && aligned(weight, 16) && aligned(bias, 16);
     JnArgs a;
     a.s = jn_shape(lx, ly, cu, packed_rows, N, T, U1, H, geo);
     a.f = f;
@@ -337,13 +334,7 @@ int ctct_b200_joint_norm_forward(const void *f, int64_t f_sn, int64_t f_st, cons
     const unsigned grid = static_cast<unsigned>(geo.blocks + (packed ? 16 : 0));
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     return with_type(dtype, [&](auto t) {
-        using E = decltype(t);
-        if (geo.P == 4)
-            jn_launch<E, 4>(geo, vec, a, grid, st);
-        else if (geo.P == 8)
-            jn_launch<E, 8>(geo, vec, a, grid, st);
-        else
-            jn_launch<E, 32>(geo, vec, a, grid, st);
+        jn_launch<decltype(t)>(geo, vec, a, grid, st);
         return check_launch("joint_norm");
     });
 }
@@ -360,16 +351,16 @@ int ctct_b200_joint_norm_backward(const void *dy, const void *f, int64_t f_sn, i
     JnGeom geo;
     if (!jn_grad_geom(N, T, U1, H, &geo)) return CTCT_ERR_UNSUPPORTED;
     const JnSaved sv = jn_saved(N, T, U1, packed_rows, 1);
-    const JnWs ws = jn_ws(N, T, U1, H, geo);
+    const JnWs ws = jn_ws(N, T, U1, H, rows, geo);
     if (rows > 0 && (!dy || (N > 0 && T > 0 && (!f || !g)))) return CTCT_ERR_ARG;
     if (rows > 0 && geo.blocks > 0 && (!saved || !aligned(saved, 256) || saved_bytes < sv.total)) return CTCT_ERR_WORKSPACE;
     if (geo.blocks > 0 && (!workspace || !aligned(workspace, 256) || workspace_bytes < ws.total)) return CTCT_ERR_WORKSPACE;
     const char *sb = static_cast<const char *>(saved);
     char *wb = static_cast<char *>(workspace);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const size_t es = esize(dtype), p_al = (param_f32 || dtype == CTCT_F32) ? 16 : 8;
-    const bool vec = H % 4 == 0 && f_sn % 4 == 0 && f_st % 4 == 0 && g_sn % 4 == 0 && g_su % 4 == 0 && aligned(f, 4 * es) &&
-                     aligned(g, 4 * es) && aligned(dy, 4 * es) && aligned(weight, p_al);
+    const int64_t E = 16 / static_cast<int64_t>(esize(dtype));
+    const bool vec = H % E == 0 && f_sn % E == 0 && f_st % E == 0 && g_sn % E == 0 && g_su % E == 0 && aligned(f, 16) && aligned(g, 16) &&
+                     aligned(dy, 16) && aligned(weight, 16);
     JnGradArgs a;
     a.s = jn_shape(lx, ly, packed && rows > 0 ? reinterpret_cast<const int64_t *>(sb + sv.cu) : nullptr, packed_rows, N, T, U1, H, geo);
     a.f = f;
@@ -384,40 +375,56 @@ int ctct_b200_joint_norm_backward(const void *dy, const void *f, int64_t f_sn, i
     a.fm = reinterpret_cast<const float *>(sb + sv.fm);
     a.gm = reinterpret_cast<const float *>(sb + sv.gm);
     a.rstd = reinterpret_cast<const float *>(sb + sv.rstd);
-    a.part_f = reinterpret_cast<float *>(wb + ws.f);
-    a.part_g = reinterpret_cast<float *>(wb + ws.g);
+    a.part_a = reinterpret_cast<float *>(wb + ws.a);
+    a.part_b = reinterpret_cast<float *>(wb + ws.b);
     a.part_w = reinterpret_cast<float *>(wb + ws.w);
-    JnReduceArgs r;
+    a.part_c = reinterpret_cast<float2 *>(wb + ws.c);
+    a.rows = rows;
+    a.slices = geo.slices;
+    const bool some = rows > 0 && geo.blocks > 0;
+    JnFinishArgs r;
     r.s = a.s;
-    r.part_f = a.part_f;
-    r.part_g = a.part_g;
+    r.f = f;
+    r.g = g;
+    r.f_sn = f_sn;
+    r.f_st = f_st;
+    r.g_sn = g_sn;
+    r.g_su = g_su;
+    r.w = weight;
+    r.p_f32 = a.p_f32;
+    r.fm = a.fm;
+    r.gm = a.gm;
+    r.rstd = a.rstd;
+    r.part_a = a.part_a;
+    r.part_b = a.part_b;
     r.part_w = a.part_w;
+    r.part_c = a.part_c;
+    r.rows = rows;
+    r.warps = geo.slices * (geo.threads / 32);
     r.df = df;
     r.dg = dg;
     r.dw = dweight;
     r.db = dbias;
-    r.p_f32 = a.p_f32;
-    const bool some = rows > 0 && geo.blocks > 0;
-    r.parts_w = some ? geo.blocks : 0;
+    r.tiles = some ? geo.blocks : 0;
     r.no_rows = !some;
-    const int64_t wb_n = 2 * ceil_div(H, 32), fb = ceil_div(N * T * H, 1024), gb = ceil_div(N * U1 * H, 1024);
-    if (wb_n + fb + gb > kMaxGrid) return CTCT_ERR_UNSUPPORTED;
-    r.w_blocks = static_cast<unsigned>(wb_n);
-    r.f_blocks = static_cast<unsigned>(fb);
+    r.w_cols = static_cast<int>(ceil_div(H, JF_W_COLS));
+    r.g_slices = static_cast<int>(ceil_div(H, JF_THREADS * JF_COLS));
+    const int64_t w_blocks = dweight || dbias ? 2 * static_cast<int64_t>(r.w_cols) : 0;
+    const int64_t g_blocks = N * ceil_div(U1, JF_ROWS) * r.g_slices, f_blocks = N * ceil_div(T, JF_ROWS) * r.g_slices;
+    if (w_blocks + g_blocks + f_blocks > kMaxGrid) return CTCT_ERR_UNSUPPORTED;
+    r.w_blocks = static_cast<unsigned>(w_blocks);
+    r.g_blocks = static_cast<unsigned>(g_blocks);
     return with_type(dtype, [&](auto t) -> int {
-        using E = decltype(t);
+        using E_ = decltype(t);
+        constexpr int VE = sizeof(E_) == 4 ? 4 : 8;
         if (some) {
-            int rc;
-            if (geo.P == 4)
-                rc = jn_launch_grad(vec ? k_joint_norm_grad<E, 4, 4, 8> : k_joint_norm_grad<E, 1, 4, 8>, geo, a, st);
-            else if (geo.P == 8)
-                rc = jn_launch_grad(vec ? k_joint_norm_grad<E, 4, 8, 4> : k_joint_norm_grad<E, 1, 8, 4>, geo, a, st);
-            else
-                rc = jn_launch_grad(vec ? k_joint_norm_grad<E, 4, 32, 1> : k_joint_norm_grad<E, 1, 32, 1>, geo, a, st);
-            if (rc) return rc;
+            auto kernel = vec ? k_joint_norm_grad<E_, VE> : k_joint_norm_grad<E_, 1>;
+            launch_pdl(kernel, dim3(static_cast<unsigned>(geo.blocks * geo.slices)), dim3(geo.threads), geo.smem, st, a);
+            if (int rc = check_launch("joint_norm_grad")) return rc;
         }
-        launch_pdl(k_joint_norm_reduce<E>, dim3(static_cast<unsigned>(wb_n + fb + gb)), dim3(1024), 0, st, r);
-        return check_launch("joint_norm_reduce");
+        if (w_blocks + g_blocks + f_blocks == 0) return CTCT_OK;
+        launch_pdl(k_joint_norm_finish<E_>, dim3(static_cast<unsigned>(w_blocks + g_blocks + f_blocks)), dim3(JF_THREADS), 0, st, r);
+        return check_launch("joint_norm_finish");
     });
 }
 

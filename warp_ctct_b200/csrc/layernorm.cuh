@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(1024) k_ln_reduce(const float *part, int64_t P
     pdl_wait();
     void *out = blockIdx.y == 0 ? dw : db;
     if (!out) return;
-    reduce_columns<T>(ReduceArgs{part + blockIdx.y * P * H, out, p_f32, P, H}, blockIdx.x, 0, sm);
+    reduce_columns<T, 32, 32>(ReduceArgs{part + blockIdx.y * P * H, out, p_f32, P, H}, blockIdx.x, 0, sm);
 }
 
 }  // namespace ctct
