@@ -313,7 +313,7 @@ def test_refusals(W):
                 lambda: W.joint_layer_norm_packed(f, g, torch.ones(2, dtype=torch.int32, device=DEV), torch.ones(2, dtype=torch.int32, device=DEV), rows=-1)):
         with pytest.raises(RuntimeError):
             bad()
-    wide = torch.zeros((1, 1, 16385), device=DEV)
+    wide = torch.zeros((1, 1, 8193), device=DEV)
     with pytest.raises(RuntimeError, match="not supported"):
         W.joint_layer_norm(wide, wide)
 

@@ -62,8 +62,8 @@ def test_joint_norm_entry_points_refuse_bad_arguments(lib):
     assert lib.ctct_b200_joint_norm_saved_bytes(2, 3, 4, -1, 0) == 0   # nothing is kept without a gradient
     assert lib.ctct_b200_joint_norm_saved_bytes(2, 3, 4, 10, 0) >= 24
     assert lib.ctct_b200_joint_norm_saved_bytes(2, 3, 4, -1, 1) >= 4 * (6 + 8 + 24)
-    assert lib.ctct_b200_joint_norm_workspace_bytes(2, 3, 4, 16385, -1) == 0
-    assert lib.ctct_b200_joint_norm_workspace_bytes(2, 3, 4, 16384, -1) > 0
+    assert lib.ctct_b200_joint_norm_workspace_bytes(2, 3, 4, 8193) == 0
+    assert lib.ctct_b200_joint_norm_workspace_bytes(2, 3, 4, 8192) > 0
 
     def fwd(f=p, g=p, dtype=0, lx=p, ly=p, N=2, T=3, U1=4, H=8, rows=-1, y=p, grad=0, saved=None, nbytes=0):
         return lib.ctct_b200_joint_norm_forward(f, T * H, H, g, U1 * H, H, dtype, lx, ly, N, T, U1, H, rows, None, None, 1, 1e-5, y,
@@ -74,7 +74,7 @@ def test_joint_norm_entry_points_refuse_bad_arguments(lib):
     assert fwd(rows=5, lx=None) == -1
     assert fwd(rows=5) == -2 and fwd(grad=1) == -2 and fwd(grad=1, saved=p, nbytes=8) == -2
     assert fwd(grad=1, saved=p + 4, nbytes=1 << 20) == -2
-    assert fwd(H=16385) == -4
+    assert fwd(H=8193) == -4
     assert fwd(N=0) == 0 and fwd(T=0) == 0 and fwd(rows=0) == 0
     bwd = lib.ctct_b200_joint_norm_backward
     ok = [p, p, 24, 8, p, 32, 8, 0, p, p, 2, 3, 4, 8, -1, p, 1, p, 1 << 20, p, p, p, p, p, 1 << 24, None]

@@ -74,7 +74,7 @@ SIGNATURES = {
     "ctct_b200_layer_norm_backward": (_int, [_vp, _i64, _vp, _i64, _int, _i64, _i64, _vp, _int, _vp, _vp, _vp, _vp, _vp, _sz,
                                              _vp]),
     "ctct_b200_joint_norm_saved_bytes": (_sz, [_i64, _i64, _i64, _i64, _int]),
-    "ctct_b200_joint_norm_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64]),
+    "ctct_b200_joint_norm_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),
     "ctct_b200_joint_norm_forward": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _int, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
                                             _vp, _vp, _int, C.c_float, _vp, _int, _vp, _sz, _vp]),
     "ctct_b200_joint_norm_backward": (_int, [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _int, _vp, _vp, _i64, _i64, _i64, _i64,

@@ -11,6 +11,9 @@
 
 using namespace ctct;
 
+#ifndef JG_REGS
+#define JG_REGS 168
+#endif
 namespace {
 
 size_t esize(int dtype) { return dtype == CTCT_F32 ? 4 : 2; }
@@ -92,14 +95,17 @@ void ln_dispatch(const LnGeom &g, bool vec, const Args &a, cudaStream_t st) {
 
 // ---- the additive joiner's layer norm ----
 struct JnGeom {
-    int P, threads, slices;
+    int P, threads;
     int tspan, uspan, tblocks, ublocks;
     int64_t blocks;
     size_t smem;
 };
 // Forward: columns per thread and frames per block: 8 x 4 up to 2048 columns (16-byte accesses of 16-bit types, at
 // most 256 threads), 32 x 1 beyond, where a row's sums need all threads of a block (a path for completeness).
-constexpr int JN_THREADS = 256, JN_WIDE_THREADS = 512;
+#ifndef JG_ACC
+#define JG_ACC 26
+#endif
+constexpr int JN_THREADS = 256;
 void jn_split(int64_t N, int64_t T, int64_t U1, int64_t tspan, int64_t uspan, JnGeom *g) {
     g->ublocks = static_cast<int>(ceil_div(U1, uspan));
     g->uspan = static_cast<int>(ceil_div(U1, g->ublocks));
@@ -109,7 +115,7 @@ void jn_split(int64_t N, int64_t T, int64_t U1, int64_t tspan, int64_t uspan, Jn
     g->blocks = N * g->tblocks * g->ublocks;
 }
 bool jn_forward_geom(int64_t N, int64_t T, int64_t U1, int64_t H, JnGeom *g) {
-    if (H < 1 || H > 32 * JN_WIDE_THREADS) return false;
+    if (H < 1 || H > CTCT_MAX_JOINT_H) return false;
     g->P = H <= 8 * JN_THREADS ? 8 : 32;
     g->threads = static_cast<int>(ceil_div(H, 32 * g->P)) * 32;
     const int TF = 32 / g->P;
@@ -118,24 +124,22 @@ bool jn_forward_geom(int64_t N, int64_t T, int64_t U1, int64_t H, JnGeom *g) {
     jn_split(N, T, U1, TF, uspan, g);
     return g->blocks <= kMaxGrid - 64;
 }
-// Backward: threads are independent, so a block has the columns that 256 threads cover and further blocks the
-// rest.  A block's contexts are as many as its accumulators' share of shared memory holds; its frames as
-// many as leave enough blocks.
+// Backward: a thread has 8 columns, a block all of a row.  A block's contexts are as many as its share of shared
+// memory holds (36 KB: six blocks of 64 threads on an SM at H = 512, as many as registers allow), its frames as many
+// as leave a dozen blocks for every SM, since utterances are of different lengths.
 bool jn_grad_geom(int64_t N, int64_t T, int64_t U1, int64_t H, JnGeom *g) {
-    if (H < 1 || H > 32 * JN_WIDE_THREADS) return false;
-    const int64_t all = ceil_div(H, 32 * JG_P) * 32;
+    if (H < 1 || H > CTCT_MAX_JOINT_H) return false;
     g->P = JG_P;
-    g->threads = static_cast<int>(all < JG_MAX_THREADS ? all : JG_MAX_THREADS);
-    g->slices = static_cast<int>(ceil_div(H, JG_P * JG_MAX_THREADS));
+    g->threads = static_cast<int>(ceil_div(H, 32 * JG_P) * 32);
     const int64_t per_context = static_cast<int64_t>(g->threads) * JG_P * 4;
-    int64_t uspan = (32 * 1024) / per_context;
+    int64_t uspan = (JG_ACC * 1024) / per_context;
     uspan = uspan < 1 ? 1 : uspan > U1 ? U1 : uspan;
     int64_t tspan = 16 * JG_TF;
-    while (tspan > JG_TF && N * ceil_div(T, tspan) * ceil_div(U1, uspan) < 16 * kSms) tspan /= 2;
+    while (tspan > JG_TF && N * ceil_div(T, tspan) * ceil_div(U1, uspan) < 12 * kSms) tspan /= 2;
     while (uspan > 1 && N * ceil_div(T, tspan) * ceil_div(U1, uspan) < kSms) uspan = (uspan + 1) / 2;
     jn_split(N, T, U1, tspan, uspan, g);
-    g->smem = static_cast<size_t>(g->uspan) * per_context;
-    return g->blocks * g->slices <= kMaxGrid;
+    g->smem = jg_smem_bytes(g->threads, g->tspan, g->uspan);
+    return g->blocks <= kMaxGrid;
 }
 bool jn_dims_ok(int64_t N, int64_t T, int64_t U1, int64_t H) {
     return N >= 0 && N <= 65535 && T >= 0 && U1 >= 1 && H >= 1 && H < (int64_t(1) << 31) && T * U1 < (int64_t(1) << 31) &&
@@ -159,15 +163,14 @@ JnSaved jn_saved(int64_t N, int64_t T, int64_t U1, int64_t packed_rows, int want
     return s;
 }
 struct JnWs {
-    size_t a, b, w, c, total;
+    size_t f, g, w, total;
 };
-JnWs jn_ws(int64_t N, int64_t T, int64_t U1, int64_t H, int64_t rows, const JnGeom &g) {
+JnWs jn_ws(int64_t N, int64_t T, int64_t U1, int64_t H, const JnGeom &g) {
     JnWs w;
-    w.a = 0;
-    w.b = align256(static_cast<size_t>(N) * g.ublocks * T * H * 4);
-    w.w = align256(w.b + static_cast<size_t>(N) * g.tblocks * U1 * H * 4);
-    w.c = align256(w.w + 2 * static_cast<size_t>(g.blocks) * H * 4);
-    w.total = align256(w.c + static_cast<size_t>(g.slices * (g.threads / 32)) * rows * 8);
+    w.f = 0;
+    w.g = align256(static_cast<size_t>(N) * g.ublocks * T * H * 4);
+    w.w = align256(w.g + static_cast<size_t>(N) * g.tblocks * U1 * H * 4);
+    w.total = align256(w.w + 2 * static_cast<size_t>(g.blocks) * H * 4);
     return w;
 }
 JnShape jn_shape(const int32_t *lx, const int32_t *ly, const int64_t *cu, int64_t packed_rows, int64_t N, int64_t T, int64_t U1,
@@ -287,10 +290,10 @@ size_t ctct_b200_joint_norm_saved_bytes(int64_t N, int64_t T, int64_t U1, int64_
     return jn_saved(N, T, U1, packed_rows, want_grad).total;
 }
 
-size_t ctct_b200_joint_norm_workspace_bytes(int64_t N, int64_t T, int64_t U1, int64_t H, int64_t packed_rows) {
+size_t ctct_b200_joint_norm_workspace_bytes(int64_t N, int64_t T, int64_t U1, int64_t H) {
     JnGeom g;
     if (!jn_dims_ok(N, T, U1, H) || !jn_grad_geom(N, T, U1, H, &g)) return 0;
-    return jn_ws(N, T, U1, H, packed_rows >= 0 ? packed_rows : N * T * U1, g).total;
+    return jn_ws(N, T, U1, H, g).total;
 }
 
 int ctct_b200_joint_norm_forward(const void *f, int64_t f_sn, int64_t f_st, const void *g, int64_t g_sn, int64_t g_su, int dtype,
@@ -351,7 +354,7 @@ int ctct_b200_joint_norm_backward(const void *dy, const void *f, int64_t f_sn, i
     JnGeom geo;
     if (!jn_grad_geom(N, T, U1, H, &geo)) return CTCT_ERR_UNSUPPORTED;
     const JnSaved sv = jn_saved(N, T, U1, packed_rows, 1);
-    const JnWs ws = jn_ws(N, T, U1, H, rows, geo);
+    const JnWs ws = jn_ws(N, T, U1, H, geo);
     if (rows > 0 && (!dy || (N > 0 && T > 0 && (!f || !g)))) return CTCT_ERR_ARG;
     if (rows > 0 && geo.blocks > 0 && (!saved || !aligned(saved, 256) || saved_bytes < sv.total)) return CTCT_ERR_WORKSPACE;
     if (geo.blocks > 0 && (!workspace || !aligned(workspace, 256) || workspace_bytes < ws.total)) return CTCT_ERR_WORKSPACE;
@@ -375,56 +378,46 @@ int ctct_b200_joint_norm_backward(const void *dy, const void *f, int64_t f_sn, i
     a.fm = reinterpret_cast<const float *>(sb + sv.fm);
     a.gm = reinterpret_cast<const float *>(sb + sv.gm);
     a.rstd = reinterpret_cast<const float *>(sb + sv.rstd);
-    a.part_a = reinterpret_cast<float *>(wb + ws.a);
-    a.part_b = reinterpret_cast<float *>(wb + ws.b);
+    a.part_f = reinterpret_cast<float *>(wb + ws.f);
+    a.part_g = reinterpret_cast<float *>(wb + ws.g);
     a.part_w = reinterpret_cast<float *>(wb + ws.w);
-    a.part_c = reinterpret_cast<float2 *>(wb + ws.c);
-    a.rows = rows;
-    a.slices = geo.slices;
     const bool some = rows > 0 && geo.blocks > 0;
-    JnFinishArgs r;
+    JnReduceArgs r;
     r.s = a.s;
-    r.f = f;
-    r.g = g;
-    r.f_sn = f_sn;
-    r.f_st = f_st;
-    r.g_sn = g_sn;
-    r.g_su = g_su;
-    r.w = weight;
-    r.p_f32 = a.p_f32;
-    r.fm = a.fm;
-    r.gm = a.gm;
-    r.rstd = a.rstd;
-    r.part_a = a.part_a;
-    r.part_b = a.part_b;
+    r.part_f = a.part_f;
+    r.part_g = a.part_g;
     r.part_w = a.part_w;
-    r.part_c = a.part_c;
-    r.rows = rows;
-    r.warps = geo.slices * (geo.threads / 32);
     r.df = df;
     r.dg = dg;
     r.dw = dweight;
     r.db = dbias;
-    r.tiles = some ? geo.blocks : 0;
+    r.p_f32 = a.p_f32;
+    r.parts_w = some ? geo.blocks : 0;
     r.no_rows = !some;
-    r.w_cols = static_cast<int>(ceil_div(H, JF_W_COLS));
-    r.g_slices = static_cast<int>(ceil_div(H, JF_THREADS * JF_COLS));
+    r.w_cols = static_cast<int>(ceil_div(H, JR_COLS));
     const int64_t w_blocks = dweight || dbias ? 2 * static_cast<int64_t>(r.w_cols) : 0;
-    const int64_t g_blocks = N * ceil_div(U1, JF_ROWS) * r.g_slices, f_blocks = N * ceil_div(T, JF_ROWS) * r.g_slices;
-    if (w_blocks + g_blocks + f_blocks > kMaxGrid) return CTCT_ERR_UNSUPPORTED;
+    const int64_t f_blocks = ceil_div(N * T, JR_THREADS / 32), g_blocks = ceil_div(N * U1, JR_THREADS / 32);
+    if (w_blocks + f_blocks + g_blocks > kMaxGrid) return CTCT_ERR_UNSUPPORTED;
     r.w_blocks = static_cast<unsigned>(w_blocks);
-    r.g_blocks = static_cast<unsigned>(g_blocks);
+    r.f_blocks = static_cast<unsigned>(f_blocks);
     return with_type(dtype, [&](auto t) -> int {
         using E_ = decltype(t);
         constexpr int VE = sizeof(E_) == 4 ? 4 : 8;
         if (some) {
-            auto kernel = vec ? k_joint_norm_grad<E_, VE> : k_joint_norm_grad<E_, 1>;
-            launch_pdl(kernel, dim3(static_cast<unsigned>(geo.blocks * geo.slices)), dim3(geo.threads), geo.smem, st, a);
+            auto kernel = geo.threads <= JG_MAX_THREADS ? (vec ? k_joint_norm_grad<E_, VE, JG_REGS> : k_joint_norm_grad<E_, 1, 168>)
+                                                        : (vec ? k_joint_norm_grad<E_, VE, 64> : k_joint_norm_grad<E_, 1, 64>);
+            // beyond 48 KB an attribute is needed; it belongs to the current device: set with the launch
+            const size_t smem = align256(geo.smem) + (vec && geo.threads <= JG_MAX_THREADS ? jg_ring_bytes(geo.threads, sizeof(E_)) : 0);
+            if (smem > 48 * 1024 &&
+                cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess)
+                return check_launch("joint_norm_grad smem attribute");
+            a.ring_offset = static_cast<int>(align256(geo.smem));
+            launch_pdl(kernel, dim3(static_cast<unsigned>(geo.blocks)), dim3(geo.threads), smem, st, a);
             if (int rc = check_launch("joint_norm_grad")) return rc;
         }
-        if (w_blocks + g_blocks + f_blocks == 0) return CTCT_OK;
-        launch_pdl(k_joint_norm_finish<E_>, dim3(static_cast<unsigned>(w_blocks + g_blocks + f_blocks)), dim3(JF_THREADS), 0, st, r);
-        return check_launch("joint_norm_finish");
+        if (w_blocks + f_blocks + g_blocks == 0) return CTCT_OK;
+        launch_pdl(k_joint_norm_reduce<E_>, dim3(static_cast<unsigned>(w_blocks + f_blocks + g_blocks)), dim3(JR_THREADS), 0, st, r);
+        return check_launch("joint_norm_reduce");
     });
 }
 

@@ -13,16 +13,17 @@
 // range of contexts: g is loaded once for TF rows, and one round of reductions (a butterfly that halves the
 // number of values with every exchange) serves TF rows.
 //
-// Backward: with r known, everything that reads dy is one pass without a dependency on a row's own sums,
+// Backward: with r known, everything that reads dy is one pass that waits for nothing,
 //   A[t] = sum_u r dy, B[u] = sum_t r dy, db = sum dy, c1 = sum_h w dy, c2 = sum_h w dy (f + g) (f, g centred)
-// and the rest follows from sums over k1 = r c1 / H and k2 = r^3 c2 / H, which is 1 / H of the data:
+// and the rest follows from k1 = r c1 / H and k2 = r^3 c2 / H, which are 1 / H of the data:
 //   df[t] = w A[t] - sum_u k1 - f[t] sum_u k2 - sum_u k2 g[u]   (dg[u] with t and u exchanged)
 //   dw    = sum_t f[t] A[t] + sum_u g[u] B[u]
-// The first kernel streams dy: a thread has P columns of TF frames, A in registers, B in shared memory at places
-// that only it touches, no barrier anywhere (a warp's share of c1 and c2 goes out by itself).  That is 7 float32
-// operations an element where the direct form takes 12 and waits for two reductions per row in
-// between.  The second kernel multiplies k2 with f and g (two small products per utterance) and adds the partial
-// sums in a fixed order: no atomics, the same bits every time.
+// A block streams the rows of TF frames and a range of contexts with a thread's P columns of A in registers and of
+// B in shared memory at places that only it touches; a warp leaves its share of c1 and c2 in shared
+// memory and goes on.  Only behind the last context the block meets, forms k1 and k2 and adds their terms.  That is
+// 7 float32 operations an element in the stream and 2 after it, where the direct form takes 12 with two
+// reductions per row to wait for in the middle.  All sums are float32 and leave as partial rows that a second
+// launch adds in a fixed order: no atomics, the same bits every time.
 #pragma once
 
 #include <type_traits>
@@ -66,12 +67,10 @@ struct JnGradArgs {
     int p_f32;
     const void *dy;
     const float *fm, *gm, *rstd;
-    float *part_a;       // [N][ublocks][T][H]
-    float *part_b;       // [N][tblocks][U1][H]
-    float *part_w;       // [2][tiles][H]: dw, db
-    float2 *part_c;      // [warps of a row][tensor rows]: {c1, c2}
-    int64_t rows;        // rows of the tensor
-    int slices;          // blocks along the columns
+    float *part_f;       // [N][ublocks][T][H]: df
+    float *part_g;       // [N][tblocks][U1][H]: dg
+    float *part_w;       // [2][gridDim.x][H]: dw, db
+    int ring_offset;     // bytes of shared memory before the ring
 };
 
 // K sums over the warp (K = 4, 8, 16) with K - 1 + log2(32 / K) exchanges: every step sends half of the values
@@ -347,25 +346,38 @@ __global__ void __maxnreg__(128) k_joint_norm(const JnArgs a) {
 
 constexpr int JG_P = 8, JG_TF = 4;      // columns per thread, frames per block of registers
 constexpr int JG_MAX_THREADS = 256;
-#ifndef JG_REGS
-#define JG_REGS 168
+constexpr int JG_BATCH = 8;             // contexts whose g is on its way together behind the stream
+// Shared memory of a block (floats): B [uspan][P / 4][team][4], private to the threads; c1 and c2 [uspan][warps][2 * TF];
+// k1 and k2 of the present frames [uspan][2 * TF]; k2 of all frames, negative, each twice [tspan / TF][uspan][2 * TF]; sums
+// of k1 and of -k2 over the frames [uspan][2].
+#ifndef JG_STAGES
+#define JG_STAGES 2
 #endif
+inline size_t jg_ring_bytes(int threads, int esize) { return static_cast<size_t>(JG_STAGES) * JG_TF * JG_P * esize * threads; }
+inline size_t jg_smem_bytes(int threads, int tspan, int uspan) {
+    return 4 * static_cast<size_t>(uspan) * (threads * JG_P + threads / 32 * 2 * JG_TF + 2 * JG_TF + tspan / JG_TF * 2 * JG_TF + 2);
+}
 
-template <typename T, int VE>
-__global__ void __maxnreg__(JG_REGS) k_joint_norm_grad(const JnGradArgs a) {
+// REGS: registers per thread; six blocks of 64 threads on an SM with 168
+template <typename T, int VE, int REGS>
+__global__ void __maxnreg__(REGS) k_joint_norm_grad(const JnGradArgs a) {
     constexpr int P = JG_P, TF = JG_TF, NV = P / VE, Q = P / 2;
-    extern __shared__ __align__(16) float acc_b[];  // [uspan][P / 4][team][4]: B of this block, private to the threads
+    extern __shared__ __align__(16) float acc_b[];
     pdl_wait();
     pdl_trigger();
     const JnShape &s = a.s;
-    const int tid = threadIdx.x, team = blockDim.x, lane = tid & 31;
-    const int slice = blockIdx.x % a.slices;
-    const unsigned tile = blockIdx.x / a.slices;
+    const int tid = threadIdx.x, team = blockDim.x, lane = tid & 31, warps = team >> 5;
+    float *const cs = acc_b + static_cast<size_t>(s.uspan) * P * team;
+    float *const ks = cs + s.uspan * warps * 2 * TF;
+    float *const k2s = ks + s.uspan * 2 * TF;
+    float *const sums = k2s + (s.tspan / TF) * s.uspan * 2 * TF;   // sums of k1 and of -k2 over the frames, per context
+    uint4 *const ring = reinterpret_cast<uint4 *>(reinterpret_cast<char *>(acc_b) + a.ring_offset) + tid;
+    const unsigned tile = blockIdx.x;
     int col[NV], at[NV];
     bool in[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        col[i] = slice * (JG_MAX_THREADS * P) + (i * team + tid) * VE;
+        col[i] = (i * team + tid) * VE;
         in[i] = col[i] < s.H;
         at[i] = in[i] ? col[i] : 0;
     }
@@ -377,6 +389,7 @@ __global__ void __maxnreg__(JG_REGS) k_joint_norm_grad(const JnGradArgs a) {
     const int64_t base = s.first_row(n);
     const int pitch = s.row_pitch(Un);
     const int64_t pitch_h = static_cast<int64_t>(pitch) * s.H;
+    const float inv_h = 1.0f / static_cast<float>(s.H);
     const F2 z2 = f2(0.0f, 0.0f);
     F2 dw[Q], db[Q];
 #pragma unroll
@@ -394,6 +407,7 @@ __global__ void __maxnreg__(JG_REGS) k_joint_norm_grad(const JnGradArgs a) {
         }
         for (int i = 0; i < (ue - u0) * (P / 4); ++i)
             *reinterpret_cast<float4 *>(acc_b + (static_cast<size_t>(i) * team + tid) * 4) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int u = tid; u < ue - u0; u += team) sums[2 * u] = 0.0f;
         const T *g = static_cast<const T *>(a.g) + n * a.g_sn;
         const float *gms = a.gm + static_cast<int64_t>(n) * s.U1;
         auto centred_g = [&](const Raw<T, VE> (&rg)[NV], float mean, F2 (&gc)[Q]) {
@@ -406,12 +420,7 @@ __global__ void __maxnreg__(JG_REGS) k_joint_norm_grad(const JnGradArgs a) {
             }
             pair_up<P>(gv, gc);
         };
-        // warps of a row, counted over all slices
-        float2 *part_c = a.part_c + static_cast<int64_t>(slice * (JG_MAX_THREADS / 32) + (tid >> 5)) * a.rows;
-        const int kl = (lane >> 2) & (TF - 1);   // the frame whose sums this lane ends up with
-        for (int t0 = ta; t0 < te; t0 += TF) {
-            const int tn = min(TF, te - t0);
-            F2 f[TF][Q], A[TF][Q];
+        auto load_f = [&](int t0, int tn, F2 (&f)[TF][Q]) {
 #pragma unroll
             for (int k = 0; k < TF; ++k) {
                 const T *fr = static_cast<const T *>(a.f) + n * a.f_sn + (t0 + k) * a.f_st;
@@ -428,20 +437,65 @@ __global__ void __maxnreg__(JG_REGS) k_joint_norm_grad(const JnGradArgs a) {
                     }
                 }
                 pair_up<P>(fv, f[k]);
+            }
+        };
+        // visit(u - u0, centred g) for the block's contexts, JG_BATCH of them on their way together
+        auto for_g = [&](auto &&visit) {
+            for (int b = u0; b < ue; b += JG_BATCH) {
+                Raw<T, VE> rg[JG_BATCH][NV];
+                float mean[JG_BATCH];
+#pragma unroll
+                for (int j = 0; j < JG_BATCH; ++j) {
+                    const int u = min(b + j, ue - 1);
+                    mean[j] = gms[u];
+#pragma unroll
+                    for (int i = 0; i < NV; ++i) rg[j][i] = load_kept<T, VE>(g + u * a.g_su + at[i]);
+                }
+#pragma unroll
+                for (int j = 0; j < JG_BATCH; ++j) {
+                    if (b + j < ue) {
+                        F2 gc[Q];
+                        centred_g(rg[j], mean[j], gc);
+                        visit(b + j - u0, gc);
+                    }
+                }
+            }
+        };
+        const int kl = (lane >> 2) & (TF - 1);   // the frame whose sums this lane ends up with
+        for (int t0 = ta; t0 < te; t0 += TF) {
+            const int tn = min(TF, te - t0);
+            F2 f[TF][Q], A[TF][Q];
+            load_f(t0, tn, f);
+#pragma unroll
+            for (int k = 0; k < TF; ++k)
 #pragma unroll
                 for (int i = 0; i < Q; ++i) A[k][i] = z2;
-            }
             int64_t row = base + static_cast<int64_t>(t0) * pitch + u0;   // of the first of the TF frames
             const T *dy[TF];
 #pragma unroll
             for (int k = 0; k < TF; ++k) dy[k] = static_cast<const T *>(a.dy) + row * s.H + k * pitch_h;
             const T *gr = g + u0 * a.g_su;
             const float *my_r = a.rstd + row + static_cast<int64_t>(kl) * pitch;
-            float *my_c = reinterpret_cast<float *>(part_c + row + static_cast<int64_t>(kl) * pitch) + (lane >> 4);
+            float *my_c = cs + (tid >> 5) * 2 * TF + (lane >> 2);   // this lane's of {c1 of TF frames, c2 of TF frames}
             // FULL: all frames and rows are there; threads without columns read column 0 with a weight of zero
             auto walk = [&](auto full_tag) {
                 constexpr bool FULL = decltype(full_tag)::value;
-                Raw<T, VE> rd[TF][NV], rg[NV];
+                constexpr bool RING = FULL && VE * sizeof(T) == 16 && REGS > 64;   // 1024 threads leave no room for it
+                Raw<T, VE> rd[RING ? 1 : TF][NV], rg[NV];
+                int p_slot = 0, c_slot = 0;
+                auto issue = [&](bool some) {
+                    if (some) {
+                        uint4 *to = ring + p_slot * (TF * NV) * team;
+#pragma unroll
+                        for (int k = 0; k < TF; ++k) {
+#pragma unroll
+                            for (int i = 0; i < NV; ++i) cp_async16(to + (k * NV + i) * team, dy[k] + at[i]);
+                            dy[k] += s.H;
+                        }
+                    }
+                    cp_async_commit();
+                    p_slot = p_slot + 1 == JG_STAGES ? 0 : p_slot + 1;
+                };
                 // frames whose row of the context is inside the tensor (a packed one may end early: zeros from there)
                 auto inside = [&](int64_t first) {
                     if (FULL) return TF;
@@ -466,8 +520,13 @@ __global__ void __maxnreg__(JG_REGS) k_joint_norm_grad(const JnGradArgs a) {
                     gr += a.g_su;
                 };
                 int kn = inside(row);
+                if constexpr (RING) {
 #pragma unroll
-                for (int k = 0; k < TF; ++k) fetch_row(k, kn);
+                    for (int i = 0; i < JG_STAGES - 1; ++i) issue(u0 + i < ue);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < TF; ++k) fetch_row(k, kn);
+                }
                 fetch_g();
                 float r_next = (FULL || kl < kn) ? *my_r : 0.0f, gmean = gms[u0];
                 float *acc = acc_b + tid * 4;
@@ -476,7 +535,6 @@ __global__ void __maxnreg__(JG_REGS) k_joint_norm_grad(const JnGradArgs a) {
                     F2 gc[Q], B[Q];
                     centred_g(rg, gmean, gc);
                     const bool more = u + 1 < ue;
-                    const int kn_now = kn;
                     ++row;
                     ++my_r;
                     if (more) {
@@ -488,14 +546,26 @@ __global__ void __maxnreg__(JG_REGS) k_joint_norm_grad(const JnGradArgs a) {
                     float v[2 * TF];
 #pragma unroll
                     for (int i = 0; i < Q; ++i) B[i] = z2;
+                    const uint4 *slot = ring + c_slot * (TF * NV) * team;
+                    if constexpr (RING) {
+                        issue(u + JG_STAGES - 1 < ue);
+                        cp_async_wait<JG_STAGES - 1>();
+                        c_slot = c_slot + 1 == JG_STAGES ? 0 : c_slot + 1;
+                    }
 #pragma unroll
                     for (int k = 0; k < TF; ++k) {
                         float dv[P];
 #pragma unroll
-                        for (int i = 0; i < NV; ++i) unpack<T, VE>(rd[k][i], dv + i * VE);
+                        for (int i = 0; i < NV; ++i) {
+                            if constexpr (RING) {
+                                const uint4 raw = slot[(k * NV + i) * team];
+                                memcpy(&rd[0][i], &raw, sizeof(rd[0][i]));
+                            }
+                            unpack<T, VE>(rd[RING ? 0 : k][i], dv + i * VE);
+                        }
                         F2 d[Q];
                         pair_up<P>(dv, d);
-                        if (more) fetch_row(k, kn);   // on its way for a whole step
+                        if (!RING && more) fetch_row(k, kn);   // on its way for a whole step
                         const float r = __shfl_sync(0xffffffffu, r_mine, 4 * k);
                         const F2 r2 = f2(r, r);
                         F2 s1 = z2, s2 = z2;
@@ -512,8 +582,11 @@ __global__ void __maxnreg__(JG_REGS) k_joint_norm_grad(const JnGradArgs a) {
                         v[TF + k] = sum2(s2);
                     }
                     const float sum = warp_sums<2 * TF>(v);
-                    if ((lane & 3) == 0 && (FULL || kl < kn_now)) *my_c = sum;
-                    my_c += 2;
+                    if ((lane & 3) == 0) {
+                        *my_c = sum;
+                        if (tid < 4 * TF) ks[(u - u0) * 2 * TF + kl] = r_mine;
+                    }
+                    my_c += warps * 2 * TF;
 #pragma unroll
                     for (int i = 0; i < P / 4; ++i, acc += 4 * team) {
                         ulonglong2 old = *reinterpret_cast<const ulonglong2 *>(acc);
@@ -528,13 +601,66 @@ __global__ void __maxnreg__(JG_REGS) k_joint_norm_grad(const JnGradArgs a) {
                 walk(std::true_type{});
             else
                 walk(std::false_type{});
+            __syncthreads();
+            for (int i = tid; i < (ue - u0) * TF; i += team) {
+                const int u = i / TF, k = i % TF;
+                const float r = ks[u * 2 * TF + k];   // left there by the stream; k1 takes its place
+                float c1 = 0.0f, c2 = 0.0f;
+                for (int p = 0; p < warps; ++p) {
+                    const float *c = cs + (u * warps + p) * 2 * TF + k;
+                    c1 += c[0];
+                    c2 += c[TF];
+                }
+                const float k1 = r * (c1 * inv_h), k2 = r * r * (r * (c2 * inv_h));
+                ks[u * 2 * TF + k] = k1;
+                ks[u * 2 * TF + TF + k] = k2;
+                float *twice = k2s + ((t0 - ta) / TF * s.uspan + u) * 2 * TF + 2 * k;
+                twice[0] = twice[1] = -k2;
+            }
+            __syncthreads();
+            for (int u = tid; u < ue - u0; u += team) {
+                const float *k1 = ks + u * 2 * TF;
+                sums[2 * u] += (k1[0] + k1[1]) + (k1[2] + k1[3]);
+            }
+            // dw takes A as it is; df = w A - sum k1 - f sum k2 - sum k2 g
+            F2 k1_sum[TF / 2], k2_sum[TF / 2];
+#pragma unroll
+            for (int k = 0; k < TF / 2; ++k) k1_sum[k] = k2_sum[k] = z2;
+#pragma unroll
+            for (int k = 0; k < TF; ++k)
+#pragma unroll
+                for (int i = 0; i < Q; ++i) {
+                    dw[i] = fma2(f[k][i], A[k][i], dw[i]);
+                    A[k][i] = mul2(w[i], A[k][i]);
+                }
+            {
+                const float *twice = k2s + (t0 - ta) / TF * s.uspan * 2 * TF;
+                for_g([&](int u, const F2 (&gc)[Q]) {
+                    const ulonglong2 p1 = *reinterpret_cast<const ulonglong2 *>(ks + u * 2 * TF);
+                    const ulonglong2 p2 = *reinterpret_cast<const ulonglong2 *>(ks + u * 2 * TF + TF);
+                    k1_sum[0] = add2(k1_sum[0], F2{p1.x});
+                    k1_sum[1] = add2(k1_sum[1], F2{p1.y});
+                    k2_sum[0] = add2(k2_sum[0], F2{p2.x});
+                    k2_sum[1] = add2(k2_sum[1], F2{p2.y});
+#pragma unroll
+                    for (int k = 0; k < TF; ++k) {
+                        const F2 m = *reinterpret_cast<const F2 *>(twice + u * 2 * TF + 2 * k);
+#pragma unroll
+                        for (int i = 0; i < Q; ++i) A[k][i] = fma2(m, gc[i], A[k][i]);
+                    }
+                });
+            }
+            float s1[TF], s2[TF];
+            unpair<TF>(k1_sum, s1);
+            unpair<TF>(k2_sum, s2);
 #pragma unroll
             for (int k = 0; k < TF; ++k) {
-                float *out = a.part_a + ((static_cast<int64_t>(n) * s.ublocks + ub) * s.T + t0 + k) * s.H;
+                float *out = a.part_f + ((static_cast<int64_t>(n) * s.ublocks + ub) * s.T + t0 + k) * s.H;
+                const F2 m1 = f2(-s1[k], -s1[k]), m2 = f2(-s2[k], -s2[k]);
+#pragma unroll
+                for (int i = 0; i < Q; ++i) A[k][i] = add2(fma2(m2, f[k][i], A[k][i]), m1);
                 float o[P];
                 unpair<P>(A[k], o);
-#pragma unroll
-                for (int i = 0; i < Q; ++i) dw[i] = fma2(f[k][i], A[k][i], dw[i]);
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
                     if (k < tn && in[i]) {
@@ -545,35 +671,76 @@ __global__ void __maxnreg__(JG_REGS) k_joint_norm_grad(const JnGradArgs a) {
                 }
             }
         }
-        for (int u = u0; u < ue; ++u) {
-            float *out = a.part_b + ((static_cast<int64_t>(n) * s.tblocks + tb) * s.U1 + u) * s.H;
-            Raw<T, VE> rg[NV];
-            F2 gc[Q], B[Q];
+        // dw takes B as it is; dg = w B - sum k1 - g sum k2 - sum k2 f, TF frames at a time
+        const int blocks = (te - ta + TF - 1) / TF;
+        for (int u = tid; u < ue - u0; u += team) {
+            float t = 0.0f;
+            for (int i = 0; i < blocks; ++i)
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                rg[i] = Raw<T, VE>{};
-                if (in[i]) rg[i] = load_kept<T, VE>(g + u * a.g_su + col[i]);
+                for (int k = 0; k < TF; ++k) t += k2s[(i * s.uspan + u) * 2 * TF + 2 * k];
+            sums[2 * u + 1] = t;
+        }
+        __syncthreads();
+        auto load_b = [&](int u, F2 (&B)[Q]) {
+            const float *acc = acc_b + (static_cast<size_t>(u) * (P / 4) * team + tid) * 4;
+#pragma unroll
+            for (int e = 0; e < P / 4; ++e) {
+                const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(acc + e * 4 * team);
+                B[2 * e] = F2{v.x};
+                B[2 * e + 1] = F2{v.y};
             }
-            centred_g(rg, gms[u], gc);
-            float o[P];
+        };
+        auto store_b = [&](int u, const F2 (&B)[Q]) {
+            float *acc = acc_b + (static_cast<size_t>(u) * (P / 4) * team + tid) * 4;
 #pragma unroll
-            for (int i = 0; i < P / 4; ++i)
-                unpack<float, 4>(*reinterpret_cast<const uint4 *>(acc_b + (static_cast<size_t>((u - u0) * (P / 4) + i) * team + tid) * 4), o + 4 * i);
-            pair_up<P>(o, B);
+            for (int e = 0; e < P / 4; ++e) *reinterpret_cast<ulonglong2 *>(acc + e * 4 * team) = make_ulonglong2(B[2 * e].v, B[2 * e + 1].v);
+        };
+        for_g([&](int u, const F2 (&gc)[Q]) {
+            F2 B[Q];
+            load_b(u, B);
+            const float k1 = sums[2 * u], k2 = sums[2 * u + 1];
+            const F2 m1 = f2(-k1, -k1), m2 = f2(k2, k2);
 #pragma unroll
-            for (int i = 0; i < Q; ++i) dw[i] = fma2(gc[i], B[i], dw[i]);
+            for (int e = 0; e < Q; ++e) {
+                dw[e] = fma2(gc[e], B[e], dw[e]);
+                B[e] = fma2(w[e], B[e], fma2(m2, gc[e], m1));
+            }
+            store_b(u, B);
+        });
+        for (int i = 0; i < blocks; ++i) {
+            F2 f[TF][Q];
+            load_f(ta + i * TF, min(TF, te - ta - i * TF), f);
+#pragma unroll 4
+            for (int u = 0; u < ue - u0; ++u) {
+                F2 B[Q];
+                load_b(u, B);
+                const float *twice = k2s + (i * s.uspan + u) * 2 * TF;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                if (in[i]) {
-                    constexpr int W = VE < 4 ? VE : 4;
+                for (int k = 0; k < TF; ++k) {
+                    const F2 m = *reinterpret_cast<const F2 *>(twice + 2 * k);
 #pragma unroll
-                    for (int e = 0; e < VE; e += W) store_raw<float, W>(out + col[i] + e, pack<float, W>(o + i * VE + e));
+                    for (int e = 0; e < Q; ++e) B[e] = fma2(m, f[k][e], B[e]);
+                }
+                if (i + 1 < blocks) {
+                    store_b(u, B);
+                } else {
+                    float *out = a.part_g + ((static_cast<int64_t>(n) * s.tblocks + tb) * s.U1 + u0 + u) * s.H;
+                    float o[P];
+                    unpair<P>(B, o);
+#pragma unroll
+                    for (int c = 0; c < NV; ++c) {
+                        if (in[c]) {
+                            constexpr int W = VE < 4 ? VE : 4;
+#pragma unroll
+                            for (int e = 0; e < VE; e += W) store_raw<float, W>(out + col[c] + e, pack<float, W>(o + c * VE + e));
+                        }
+                    }
                 }
             }
         }
     }
     float *pw = a.part_w + static_cast<int64_t>(tile) * s.H;
-    float *pb = pw + static_cast<int64_t>(gridDim.x / a.slices) * s.H;
+    float *pb = pw + static_cast<int64_t>(gridDim.x) * s.H;
     float ow[P], ob[P];
     unpair<P>(dw, ow);
     unpair<P>(db, ob);
@@ -590,198 +757,65 @@ __global__ void __maxnreg__(JG_REGS) k_joint_norm_grad(const JnGradArgs a) {
     }
 }
 
-// Second half of the backward pass, three kinds of blocks: [0, w_blocks) add up dw and db, then JF_ROWS contexts
-// of dg each, then JF_ROWS frames of df each.  A frame t >= lx and a context u > ly get zeros.
-constexpr int JF_ROWS = 8, JF_CHUNK = 64, JF_THREADS = 128, JF_COLS = 4, JF_BATCH = 8;  // 512 columns a block
-constexpr int JF_W_COLS = 8;  // columns of a block that adds up dw or db: whole 32-byte sectors, 16 partials at a time
-struct JnFinishArgs {
+// The partial sums of k_joint_norm_grad, three kinds of blocks: [0, w_blocks) dw and db, then df, then dg, a warp per
+// row.  A frame that no range of contexts has touched (t >= lx) and a context beyond ly get zeros.
+constexpr int JR_THREADS = 256, JR_COLS = 8;   // JR_COLS columns of dw or db a block: whole 32-byte sectors, 32 partials at a time
+struct JnReduceArgs {
     JnShape s;
-    const void *f, *g;
-    int64_t f_sn, f_st, g_sn, g_su;
-    const void *w;
-    int p_f32;
-    const float *fm, *gm, *rstd;
-    const float *part_a, *part_b, *part_w;
-    const float2 *part_c;
-    int64_t rows;
-    int warps;                 // shares of c1 and c2 per row
+    const float *part_f, *part_g, *part_w;
     void *df, *dg, *dw, *db;   // any of them nullptr
-    int64_t tiles;             // partial rows of dw and db
+    int p_f32;
+    int64_t parts_w;           // blocks of the gradient launch
     int no_rows;               // there was none: every gradient is zero
-    unsigned w_blocks, g_blocks;
-    int w_cols, g_slices;      // blocks along the columns of dw and db; of df and dg
+    unsigned w_blocks, f_blocks;
+    int w_cols;                // blocks along the columns of dw, and of db
 };
-
-// df of JF_ROWS frames ("own" rows; "other" are the contexts) or dg of JF_ROWS contexts (the other way round)
 template <typename T>
-__device__ __forceinline__ void joint_norm_finish_rows(const JnFinishArgs &a, bool is_f, unsigned block) {
-    __shared__ __align__(16) float k1s[JF_CHUNK][JF_ROWS], k2s[JF_CHUNK][JF_ROWS];
-    __shared__ float means[JF_CHUNK], totals[2][JF_ROWS];
-    const JnShape &s = a.s;
-    const int tid = threadIdx.x, team = blockDim.x;
-    const int rows = is_f ? s.T : s.U1;
-    const int groups = (rows + JF_ROWS - 1) / JF_ROWS;
-    const int slice = block % a.g_slices;
-    const unsigned q = block / a.g_slices;
-    const int n = static_cast<int>(q / groups), i0 = static_cast<int>(q - static_cast<unsigned>(n) * groups) * JF_ROWS;
-    const int Tn = a.no_rows ? 0 : s.frames(n), Un = a.no_rows ? 0 : s.contexts(n);
-    const int others = is_f ? Un : Tn;
-    const int own = others > 0 ? (is_f ? Tn : Un) - i0 : 0;   // own rows that take part: nothing is known of the rest
-    const int col = (slice * team + tid) * JF_COLS;     // JF_COLS neighbours; the last thread of a row may have fewer
-    const int cols = min(max(s.H - col, 0), JF_COLS);
-    const bool vec = (s.H | (is_f ? a.g_su | a.g_sn : a.f_st | a.f_sn)) % JF_COLS == 0 &&
-                     reinterpret_cast<uintptr_t>(is_f ? a.g : a.f) % (JF_COLS * sizeof(T)) == 0;
-    const int64_t base = s.first_row(n);
-    const int pitch = s.row_pitch(Un);
-    const int64_t si = is_f ? pitch : 1, sj = is_f ? 1 : pitch;
-    const float inv_h = 1.0f / static_cast<float>(s.H);
-    const float *other_mean = is_f ? a.gm + static_cast<int64_t>(n) * s.U1 : a.fm + static_cast<int64_t>(n) * s.T;
-    const T *other = is_f ? static_cast<const T *>(a.g) + n * a.g_sn : static_cast<const T *>(a.f) + n * a.f_sn;
-    const int64_t other_st = is_f ? a.g_su : a.f_st;
-    F2 acc[JF_ROWS][2];
-#pragma unroll
-    for (int k = 0; k < JF_ROWS; ++k) acc[k][0] = acc[k][1] = f2(0.0f, 0.0f);
-    if (tid < 2 * JF_ROWS) totals[tid / JF_ROWS][tid % JF_ROWS] = 0.0f;
-    for (int j0 = 0; own > 0 && j0 < others; j0 += JF_CHUNK) {
-        const int jn = min(JF_CHUNK, others - j0);
-        __syncthreads();
-        // lanes along the axis whose rows are neighbours in memory: contexts
-#pragma unroll 2
-        for (int i = tid; i < JF_ROWS * JF_CHUNK; i += team) {
-            const int k = is_f ? i / JF_CHUNK : i % JF_ROWS, j = is_f ? i % JF_CHUNK : i / JF_ROWS;
-            const int64_t row = base + (i0 + k) * si + (j0 + j) * sj;
-            float k1 = 0.0f, k2 = 0.0f;
-            if (k < own && j < jn && (!s.cu || row < s.packed_rows)) {
-                float c1 = 0.0f, c2 = 0.0f;
-                const float r = a.rstd[row];
-#pragma unroll 2
-                for (int p = 0; p < a.warps; ++p) {
-                    const float2 c = a.part_c[p * a.rows + row];
-                    c1 += c.x;
-                    c2 += c.y;
-                }
-                k1 = r * (c1 * inv_h);
-                k2 = r * r * (r * (c2 * inv_h));
-            }
-            k1s[j][k] = k1;
-            k2s[j][k] = k2;
-        }
-        for (int j = tid; j < JF_CHUNK; j += team) means[j] = j < jn ? other_mean[j0 + j] : 0.0f;
-        __syncthreads();
-        if (tid < 2 * JF_ROWS * 4) {   // four lanes per own row and sum
-            const float(*from)[JF_ROWS] = tid < JF_ROWS * 4 ? k1s : k2s;
-            const int k = (tid >> 2) % JF_ROWS;
-            float t = 0.0f;
-            for (int j = tid & 3; j < JF_CHUNK; j += 4) t += from[j][k];
-            t += __shfl_xor_sync(0xffffffffu, t, 1);
-            t += __shfl_xor_sync(0xffffffffu, t, 2);
-            if ((tid & 3) == 0) totals[tid >= JF_ROWS * 4][k] += t;
-        }
-        if (cols > 0) {
-            for (int j1 = 0; j1 < jn; j1 += JF_BATCH) {   // a batch of rows is on its way together
-                float x[JF_BATCH][JF_COLS];
-                Raw<T, JF_COLS> raw[JF_BATCH];
-#pragma unroll
-                for (int b = 0; b < JF_BATCH; ++b) {
-                    // behind the last row: that row again, with a factor of zero
-                    const T *p = other + static_cast<int64_t>(min(j0 + j1 + b, others - 1)) * other_st + col;
-                    if (vec) {
-                        raw[b] = load_kept<T, JF_COLS>(p);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < JF_COLS; ++e) x[b][e] = e < cols ? to_float(p[e]) : 0.0f;
-                    }
-                }
-#pragma unroll
-                for (int b = 0; b < JF_BATCH; ++b) {
-                    if (vec) unpack<T, JF_COLS>(raw[b], x[b]);
-                    const float mean = j1 + b < jn ? means[j1 + b] : 0.0f;
-                    const F2 m = f2(-mean, -mean);
-                    const F2 x0 = add2(f2(x[b][0], x[b][1]), m), x1 = add2(f2(x[b][2], x[b][3]), m);
-                    float k2[JF_ROWS];
-                    unpack<float, 4>(*reinterpret_cast<const uint4 *>(&k2s[j1 + b][0]), k2);
-                    unpack<float, 4>(*reinterpret_cast<const uint4 *>(&k2s[j1 + b][4]), k2 + 4);
-#pragma unroll
-                    for (int k = 0; k < JF_ROWS; ++k) {
-                        const F2 kk = f2(k2[k], k2[k]);
-                        acc[k][0] = fma2(kk, x0, acc[k][0]);
-                        acc[k][1] = fma2(kk, x1, acc[k][1]);
-                    }
-                }
-            }
-        }
-    }
-    __syncthreads();
-    if (cols <= 0) return;
-    const int parts = own > 0 ? (others + (is_f ? s.uspan : s.tspan) - 1) / (is_f ? s.uspan : s.tspan) : 0;
-    const int parts_all = is_f ? s.ublocks : s.tblocks;
-    const int64_t plane = static_cast<int64_t>(rows) * s.H;
-    const float *part = (is_f ? a.part_a : a.part_b) + static_cast<int64_t>(n) * parts_all * plane + static_cast<int64_t>(i0) * s.H + col;
-    T *out = static_cast<T *>(is_f ? a.df : a.dg) + (static_cast<int64_t>(n) * rows + i0) * s.H + col;
-    const T *mine = (is_f ? static_cast<const T *>(a.f) + n * a.f_sn + i0 * a.f_st : static_cast<const T *>(a.g) + n * a.g_sn + i0 * a.g_su) + col;
-    const int64_t mine_st = is_f ? a.f_st : a.g_su;
-    const float *own_mean = (is_f ? a.fm + static_cast<int64_t>(n) * s.T : a.gm + static_cast<int64_t>(n) * s.U1) + i0;
-    float w[JF_COLS];
-#pragma unroll
-    for (int e = 0; e < JF_COLS; ++e) {
-        w[e] = 1.0f;
-        if (a.w && e < cols) load_param<T, 1>(a.w, a.p_f32, col + e, w + e);
-    }
-#pragma unroll
-    for (int k = 0; k < JF_ROWS; ++k) {
-        if (i0 + k >= rows) break;
-        float x[JF_COLS];
-        split(acc[k][0], x[0], x[1]);
-        split(acc[k][1], x[2], x[3]);
-        float sum[JF_COLS] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (k < own) {
-#pragma unroll 4
-            for (int p = 0; p < parts; ++p) {
-                const float *from = part + p * plane + static_cast<int64_t>(k) * s.H;
-                if (s.H % JF_COLS == 0) {
-                    float v[JF_COLS];
-                    unpack<float, 4>(*reinterpret_cast<const uint4 *>(from), v);
-#pragma unroll
-                    for (int e = 0; e < JF_COLS; ++e) sum[e] += v[e];
-                } else {
-#pragma unroll
-                    for (int e = 0; e < JF_COLS; ++e)
-                        if (e < cols) sum[e] += from[e];
-                }
-            }
-            const float t1 = totals[0][k], t2 = totals[1][k], mean = own_mean[k];
-#pragma unroll
-            for (int e = 0; e < JF_COLS; ++e) {
-                const float c = e < cols ? to_float(mine[k * mine_st + e]) - mean : 0.0f;
-                sum[e] = fmaf(w[e], sum[e], -t1) - fmaf(c, t2, x[e]);
-            }
-        }
-        if (s.H % JF_COLS == 0) {
-            store_raw<T, JF_COLS>(out + static_cast<int64_t>(k) * s.H, pack<T, JF_COLS>(sum));
-        } else {
-#pragma unroll
-            for (int e = 0; e < JF_COLS; ++e)
-                if (e < cols) out[static_cast<int64_t>(k) * s.H + e] = from_float<T>(sum[e]);
-        }
-    }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(JF_THREADS) k_joint_norm_finish(const JnFinishArgs a) {
+__global__ void __launch_bounds__(JR_THREADS) k_joint_norm_reduce(const JnReduceArgs a) {
     pdl_wait();
+    const JnShape &s = a.s;
     if (blockIdx.x < a.w_blocks) {
-        __shared__ float sm[JF_THREADS / JF_W_COLS][JF_W_COLS + 1];
+        __shared__ float sm[JR_THREADS / JR_COLS][JR_COLS + 1];
         const int which = blockIdx.x / a.w_cols;
         void *out = which ? a.db : a.dw;
         if (out)
-            reduce_columns<T, JF_W_COLS, JF_THREADS / JF_W_COLS>(ReduceArgs{a.part_w + which * a.tiles * a.s.H, out, a.p_f32, a.tiles, a.s.H},
-                                               blockIdx.x - which * a.w_cols, 0, sm);
+            reduce_columns<T, JR_COLS, JR_THREADS / JR_COLS>(ReduceArgs{a.part_w + which * a.parts_w * s.H, out, a.p_f32, a.parts_w, s.H},
+                                                             blockIdx.x - which * a.w_cols, 0, sm);
         return;
     }
-    const unsigned block = blockIdx.x - a.w_blocks;
-    const bool is_f = block >= a.g_blocks;
-    if (!(is_f ? a.df : a.dg)) return;
-    joint_norm_finish_rows<T>(a, is_f, is_f ? block - a.g_blocks : block);
+    const bool is_f = blockIdx.x < a.w_blocks + a.f_blocks;
+    const int rows = is_f ? s.T : s.U1, parts_all = is_f ? s.ublocks : s.tblocks;
+    void *out = is_f ? a.df : a.dg;
+    const unsigned i = (blockIdx.x - a.w_blocks - (is_f ? 0 : a.f_blocks)) * (JR_THREADS / 32) + (threadIdx.x >> 5);
+    if (!out || i >= static_cast<unsigned>(rows) * s.N) return;
+    const int n = static_cast<int>(i / rows), r = static_cast<int>(i - static_cast<unsigned>(n) * rows);
+    const int Tn = a.no_rows ? 0 : s.frames(n), Un = a.no_rows ? 0 : s.contexts(n);
+    const int along = is_f ? Un : Tn, span = is_f ? s.uspan : s.tspan;
+    const int parts = r < (is_f ? Tn : Un) ? (along + span - 1) / span : 0;
+    const int64_t plane = static_cast<int64_t>(rows) * s.H;
+    const float *p = (is_f ? a.part_f : a.part_g) + static_cast<int64_t>(n) * parts_all * plane + static_cast<int64_t>(r) * s.H;
+    T *o = static_cast<T *>(out) + static_cast<int64_t>(i) * s.H;
+    if (s.H % 4 == 0) {   // both buffers are whole vectors apart
+        for (int col = (threadIdx.x & 31) * 4; col < s.H; col += 128) {
+            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+            for (int k = 0; k < parts; ++k) {
+                const float4 v = *reinterpret_cast<const float4 *>(p + k * plane + col);
+                x[0] += v.x;
+                x[1] += v.y;
+                x[2] += v.z;
+                x[3] += v.w;
+            }
+            store_raw<T, 4>(o + col, pack<T, 4>(x));
+        }
+    } else {
+        for (int col = threadIdx.x & 31; col < s.H; col += 32) {
+            float sum = 0.0f;
+#pragma unroll 8
+            for (int k = 0; k < parts; ++k) sum += p[k * plane + col];
+            o[col] = from_float<T>(sum);
+        }
+    }
 }
 
 }  // namespace ctct

@@ -186,7 +186,7 @@ class JointLayerNorm(torch.autograd.Function):
             dg = torch.empty((N, U1, H), dtype=f.dtype, device=dev) if need_g else None
             dw = torch.empty((H,), dtype=weight.dtype, device=dev) if need_w else None
             db = torch.empty((H,), dtype=bias_dtype, device=dev) if need_b else None
-            nbytes = lib.ctct_b200_joint_norm_workspace_bytes(N, Tm, U1, H, rows)
+            nbytes = lib.ctct_b200_joint_norm_workspace_bytes(N, Tm, U1, H)
             ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
             rc = lib.ctct_b200_joint_norm_backward(
                 dy.data_ptr(), f.data_ptr(), f.stride(0), f.stride(1), g.data_ptr(), g.stride(0), g.stride(1),
