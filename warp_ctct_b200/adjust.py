@@ -138,7 +138,7 @@ class AdjustLogits(torch.autograd.Function):
             db = torch.empty(bias_shape, dtype=c.bias_dtype, device=dev) if need_b else None
             ws, nbytes = None, 0
             if need_b:
-                nbytes = lib.ctct_b200_adjust_workspace_bytes(c.N, c.T, c.U1, c.V)
+                nbytes = lib.ctct_b200_adjust_workspace_bytes(c.N, c.T, c.U1, c.V, c.bias_kind)
                 ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
             rc = lib.ctct_b200_adjust_backward(
                 dy.data_ptr(), _lib.ptr(logits), c.row_stride, _lib.dtype_code(dtype), _lib.ptr(tokens), c.pitch,

@@ -23,11 +23,12 @@ namespace ctct {
 
 constexpr int ADJ_THREADS = 256;
 constexpr int ADJ_UNROLL = 4;   // frames whose loads are in flight together
+constexpr int ADJ_PRE = 4;      // tokens of a step's history that a thread asks for before anything else
 
 struct AdjArgs {
     const void *x;             // logits; in the backward pass needed only where rho != 1
     int64_t x_sn;              // elements from row to row of a step's (N,V) logits (T = U1 = 1); unused otherwise
-    const int *tokens;         // step: histories (N, L); joint: labels (N, U1 - 1); or nullptr
+    const int *tokens;         // step: histories (N, L); joint: labels (N, U1 - 1); nullptr: none, or nothing to do with them
     const int *tokens_len;     // step: tokens per history; joint: nullptr (context u has u)
     int64_t L;                 // row pitch of `tokens`
     const int *lx, *ly;        // frames, labels per utterance, or nullptr: all
@@ -49,9 +50,16 @@ struct AdjArgs {
     unsigned main_blocks;      // blocks beyond it clear packed rows behind the last utterance
 };
 
-template <typename T, int VE, bool GRAD>
-__global__ void __launch_bounds__(ADJ_THREADS) k_adjust(const AdjArgs a) {
-    __shared__ int count[ADJ_THREADS * VE];
+// A thread's elements: NV chunks of VE neighbours, threads * VE apart.  STEP: one row per n (T = U1 = 1), without the
+// walk over frames and with more elements per thread, since there the set-up of a block is most of its work.
+// Four blocks of 256 threads on an SM (64 registers): with three the f32 step over 1.1 GB took 396 us
+// backward instead of 338.
+template <typename T, int VE, int NV, bool GRAD, bool STEP>
+__global__ void __launch_bounds__(ADJ_THREADS, 4) k_adjust(const AdjArgs a) {
+    constexpr int NE = VE * NV, UNROLL = STEP ? 1 : ADJ_UNROLL;
+    constexpr bool STAGE = GRAD && !STEP && VE * sizeof(T) == 16;   // logits beside repeated tokens go through shared memory
+    __shared__ __align__(16) int count[ADJ_THREADS * NE];
+    __shared__ uint4 xs[STAGE ? UNROLL * ADJ_THREADS : 1];
     pdl_wait();
     pdl_trigger();
     const int tid = threadIdx.x, threads = blockDim.x;
@@ -63,136 +71,241 @@ __global__ void __launch_bounds__(ADJ_THREADS) k_adjust(const AdjArgs a) {
             store_raw<T, VE>(out + i, zero);
         return;
     }
-    const int tile = blockIdx.x % a.tiles, q = blockIdx.x / a.tiles;
-    const int chunk = q % a.chunks;
-    const int64_t n = q / a.chunks;
-    const int Tn = a.lx ? max(0, min(a.lx[n], a.T)) : a.T;
-    const int Un = a.ly ? max(0, min(a.ly[n], a.U1 - 1)) + 1 : a.U1;
-    const unsigned V = a.V, plane = static_cast<unsigned>(a.U1) * V;  // below 2^31
-    const unsigned tile0 = static_cast<unsigned>(tile) * threads * VE;
-    const unsigned at = tile0 + tid * VE;          // this thread's first element of the plane
-    const int u_first = static_cast<int>(tile0 / V);
-    const int u_last = min(static_cast<int>((min(tile0 + threads * VE, plane) - 1) / V), Un - 1);
-    const int ta = chunk * a.tspan, tb = min(ta + a.tspan, a.T), te = max(ta, min(tb, Tn));
+    const unsigned q = blockIdx.x / static_cast<unsigned>(a.tiles), tile = blockIdx.x - q * a.tiles;
+    const int chunk = STEP ? 0 : q % static_cast<unsigned>(a.chunks);
+    const int64_t n = STEP ? q : q / static_cast<unsigned>(a.chunks);
+    // Everything that needs no other load is asked for first, so that a block of a decoder's step pays one memory
+    // latency, not a chain of them.
+    const int *tok = a.tokens ? a.tokens + n * a.L : nullptr;
+    int pre[ADJ_PRE], step_len = 0;
+    if (tok && a.tokens_len) {
+        step_len = a.tokens_len[n];
+#pragma unroll
+        for (int i = 0; i < ADJ_PRE; ++i) pre[i] = tid + i * threads < a.L ? __ldg(tok + tid + i * threads) : -1;
+    }
+    const float rho = a.rho_n ? a.rho_n[n] : a.rho;
+    const float presence = a.presence_n ? a.presence_n[n] : a.presence;
+    const float frequency = a.frequency_n ? a.frequency_n[n] : a.frequency;
+    const int Tn = STEP ? 1 : a.lx ? max(0, min(a.lx[n], a.T)) : a.T;
+    const int Un = STEP ? 1 : a.ly ? max(0, min(a.ly[n], a.U1 - 1)) + 1 : a.U1;
+    const unsigned V = a.V, plane = STEP ? V : static_cast<unsigned>(a.U1) * V;  // below 2^31
+    const unsigned tile0 = tile * threads * NE, tile1 = min(tile0 + threads * NE, plane);
+    const int u_first = STEP ? 0 : static_cast<int>(tile0 / V);
+    const int u_last = STEP ? 0 : min(static_cast<int>((tile1 - 1) / V), Un - 1);
+    const int ta = STEP ? 0 : chunk * a.tspan, tb = STEP ? 1 : min(ta + a.tspan, a.T), te = max(ta, min(tb, Tn));
     const bool work = u_first < Un && ta < te;
-    float rho = a.rho, presence = a.presence, frequency = a.frequency;
-    if (a.rho_n) rho = a.rho_n[n];
-    if (a.presence_n) presence = a.presence_n[n];
-    if (a.frequency_n) frequency = a.frequency_n[n];
-    const bool history = work && a.tokens && (rho != 1.0f || (!GRAD && (presence != 0.0f || frequency != 0.0f)));
-    if (history) {  // the same for the whole block
-        for (int i = tid; i < threads * VE; i += threads) count[i] = 0;
-        __syncthreads();
-        const int *tok = a.tokens + n * a.L;
-        for (int u = u_first; u <= u_last; ++u) {
-            const int len = a.tokens_len ? max(0, min(a.tokens_len[n], static_cast<int>(a.L))) : u;
-            const int row = static_cast<int>(u * V - tile0);  // may be negative: the tile may begin inside the row
-            for (int j = tid; j < len; j += threads) {
-                const int v = tok[j];
-                if (v < 0 || v >= a.V) continue;  // no token: ignored
-                const int to = row + v;
-                if (to >= 0 && to < threads * VE) atomicAdd(count + to, 1);
-            }
-        }
-        __syncthreads();
-    }
-    if (at >= plane) return;
-    const int u = static_cast<int>(at / V), v0 = static_cast<int>(at - u * V);
-    const bool row_ok = u < Un;
-    float add[VE];
-    unsigned hit = 0, ok = 0;
-#pragma unroll
-    for (int e = 0; e < VE; ++e) add[e] = 0.0f;
-    if (work && row_ok) {
-        if (!GRAD && a.bias) load_param<T, VE>(a.bias, a.bias_f32, n * a.bias_sn + u * a.bias_su + v0, add);
-        ok = (1u << VE) - 1;
-        if (a.allowed) ok &= a.allowed[n * a.mask_sn + u * a.mask_su + (v0 >> 5)] >> (v0 & 31);
-        if (history) {
-#pragma unroll
-            for (int e = 0; e < VE; ++e) {
-                const int c = count[tid * VE + e];
-                if (c > 0) {
-                    hit |= 1u << e;
-                    add[e] -= presence + frequency * static_cast<float>(c);
-                }
-            }
-        }
-    }
-    const float inv_rho = 1.0f / rho;
-    const bool scaled = hit && rho != 1.0f;
     // rows of this thread's elements: one every `pitch` elements
-    const int64_t base = a.cu ? a.cu[n] * a.V : static_cast<int64_t>(n) * a.T * plane;
-    const int64_t pitch = a.cu ? static_cast<int64_t>(Un) * a.V : static_cast<int64_t>(plane);
-    const T *x = static_cast<const T *>(a.x), *dy = static_cast<const T *>(a.dy);
-    const int64_t x_base = a.x_sn ? n * a.x_sn : base;
-    int t_stop = row_ok ? te : ta;
-    if (a.cu && row_ok) {   // rows beyond the packed tensor are not touched
-        const int64_t rows_left = a.packed_rows - a.cu[n] - u;   // t * Un < rows_left
-        const int64_t fit = rows_left > 0 ? (rows_left + Un - 1) / Un : 0;
-        if (fit < t_stop) t_stop = static_cast<int>(fit);
-    }
-    float db[VE];
+    const bool packed = !STEP && a.cu;
+    const int64_t base = packed ? a.cu[n] * a.V : STEP ? n * V : n * a.T * static_cast<int64_t>(plane);
+    const int64_t pitch = packed ? static_cast<int64_t>(Un) * a.V : static_cast<int64_t>(plane);
+    const T *x = static_cast<const T *>(a.x) + (a.x_sn ? n * a.x_sn : base);
+    const T *dy = static_cast<const T *>(a.dy) + base;
+    unsigned at[NV];       // place in the plane
+    int u[NV], v0[NV], t_stop[NV];
+    float add[NE];
+    unsigned ok = 0;
 #pragma unroll
-    for (int e = 0; e < VE; ++e) db[e] = 0.0f;
+    for (int c = 0; c < NV; ++c) {
+        at[c] = tile0 + (c * threads + tid) * VE;
+        u[c] = STEP ? 0 : static_cast<int>(at[c] / V);
+        v0[c] = static_cast<int>(at[c] - u[c] * V);
+        t_stop[c] = work && at[c] < plane && u[c] < Un ? te : ta;
+        if (packed && t_stop[c] > ta) {   // rows beyond the packed tensor are not touched: t * Un < rows_left
+            const int64_t rows_left = a.packed_rows - a.cu[n] - u[c];
+            const int64_t fit = rows_left > 0 ? (rows_left + Un - 1) / Un : 0;
+            if (fit < t_stop[c]) t_stop[c] = static_cast<int>(max(fit, static_cast<int64_t>(ta)));
+        }
+#pragma unroll
+        for (int e = 0; e < VE; ++e) add[c * VE + e] = 0.0f;
+        if (t_stop[c] > ta) {
+            if (!GRAD && a.bias) load_param<T, VE>(a.bias, a.bias_f32, n * a.bias_sn + u[c] * a.bias_su + v0[c], add + c * VE);
+            unsigned bits = (1u << VE) - 1;
+            if (a.allowed) bits &= a.allowed[n * a.mask_sn + u[c] * a.mask_su + (v0[c] >> 5)] >> (v0[c] & 31);
+            ok |= bits << (c * VE);
+        }
+    }
+    // the stream: logits forward, their adjusted values' gradient backward, ADJ_UNROLL frames on their way
+    const T *from = GRAD ? dy : x;
+    Raw<T, VE> in[UNROLL][NV];
+    auto fetch = [&](int t) {
+#pragma unroll
+        for (int k = 0; k < UNROLL; ++k)
+#pragma unroll
+            for (int c = 0; c < NV; ++c)
+                if (t + k < t_stop[c]) in[k][c] = load_once<T, VE>(from + (t + k) * pitch + at[c]);
+    };
+    fetch(ta);
+    const bool history = work && tok;
+    if (history) {  // the same for the whole block
+        if (NE % 4 == 0) {
+            for (int i = tid; i < threads * NE / 4; i += threads) reinterpret_cast<int4 *>(count)[i] = make_int4(0, 0, 0, 0);
+        } else {
+            for (int i = tid; i < threads * NE; i += threads) count[i] = 0;
+        }
+        __syncthreads();
+        auto note = [&](int row, int v) {   // `row`: place of the row's first element in the tile, may be negative
+            if (v < 0 || v >= a.V) return;  // no token: ignored
+            const int to = row + v;
+            if (to >= 0 && to < threads * NE) atomicAdd(count + to, 1);
+        };
+        if (STEP || a.tokens_len) {
+            const int len = max(0, min(step_len, static_cast<int>(a.L)));
+#pragma unroll
+            for (int i = 0; i < ADJ_PRE; ++i)
+                if (tid + i * threads < len) note(-static_cast<int>(tile0), pre[i]);
+            for (int j = tid + ADJ_PRE * threads; j < len; j += threads) note(-static_cast<int>(tile0), tok[j]);
+        } else {
+            for (int r = u_first; r <= u_last; ++r)
+                for (int j = tid; j < r; j += threads) note(static_cast<int>(r * V - tile0), tok[j]);
+        }
+        __syncthreads();
+    }
+    unsigned hit = 0;
+    if (history) {
+#pragma unroll
+        for (int c = 0; c < NV; ++c) {
+            constexpr int W = VE < 4 ? VE : 4;
+#pragma unroll
+            for (int e = 0; e < VE; e += W) {
+                int times[W];
+                memcpy(times, __builtin_assume_aligned(&count[(c * threads + tid) * VE + e], 4 * W), sizeof(times));
+#pragma unroll
+                for (int i = 0; i < W; ++i)
+                    if (times[i] > 0) {
+                        hit |= 1u << (c * VE + e + i);
+                        add[c * VE + e + i] -= presence + frequency * static_cast<float>(times[i]);
+                    }
+            }
+        }
+    }
+    const bool scaled = hit && rho != 1.0f;
+    const float inv_rho = scaled ? 1.0f / rho : 1.0f;
+    float db[GRAD ? NE : 1];
+#pragma unroll
+    for (int e = 0; e < (GRAD ? NE : 1); ++e) db[e] = 0.0f;
     const float ninf = -__int_as_float(0x7f800000);
-    for (int t = ta; t < t_stop; t += ADJ_UNROLL) {
-        Raw<T, VE> in[ADJ_UNROLL], grad[ADJ_UNROLL];
+    int t_end = ta;
 #pragma unroll
-        for (int k = 0; k < ADJ_UNROLL; ++k) {
-            if (t + k < t_stop) {
-                const int64_t o = (t + k) * pitch + at;
-                if (GRAD) grad[k] = load_once<T, VE>(dy + base + o);
-                if (!GRAD || (scaled && out)) in[k] = load_once<T, VE>(x + x_base + o);
-            }
+    for (int c = 0; c < NV; ++c) t_end = max(t_end, t_stop[c]);
+    for (int t = ta; t < t_end; t += UNROLL) {
+        if (t > ta) fetch(t);
+        if (STAGE && scaled && out) {   // a thread reads back what it copied itself: no barrier, and no registers
+#pragma unroll
+            for (int k = 0; k < UNROLL; ++k)
+                if (t + k < t_stop[0]) cp_async16(xs + k * ADJ_THREADS + tid, x + (t + k) * pitch + at[0]);
+            cp_async_commit();
+            cp_async_wait<0>();
         }
 #pragma unroll
-        for (int k = 0; k < ADJ_UNROLL; ++k) {
-            if (t + k < t_stop) {
-                float z[VE], g[VE];
-                if (GRAD) {
-                    unpack<T, VE>(grad[k], g);
+        for (int k = 0; k < UNROLL; ++k)
 #pragma unroll
-                    for (int e = 0; e < VE; ++e) {
-                        g[e] = (ok >> e & 1u) ? g[e] : 0.0f;
-                        db[e] += g[e];
+            for (int c = 0; c < NV; ++c)
+                if (t + k < t_stop[c]) {
+                    const int64_t o = (t + k) * pitch + at[c];
+                    float z[VE], g[VE];
+                    unpack<T, VE>(in[k][c], z);
+                    if (GRAD) {
+#pragma unroll
+                        for (int e = 0; e < VE; ++e) {
+                            g[e] = (ok >> (c * VE + e) & 1u) ? z[e] : 0.0f;
+                            db[(GRAD ? c * VE + e : 0)] += g[e];
+                        }
+                        if (!out) continue;
+                        if (scaled) {   // only the few chunks that hold a repeated token
+                            Raw<T, VE> rx;
+                            if constexpr (STAGE)
+                                memcpy(&rx, &xs[k * ADJ_THREADS + tid], sizeof(rx));
+                            else
+                                rx = load_once<T, VE>(x + o);
+                            unpack<T, VE>(rx, z);
+#pragma unroll
+                            for (int e = 0; e < VE; ++e)
+                                if ((hit & ok) >> (c * VE + e) & 1u) g[e] *= z[e] > 0.0f ? inv_rho : rho;
+                        }
+                    } else {
+                        if (scaled) {
+#pragma unroll
+                            for (int e = 0; e < VE; ++e)
+                                if (hit >> (c * VE + e) & 1u) z[e] *= z[e] > 0.0f ? inv_rho : rho;
+                        }
+#pragma unroll
+                        for (int e = 0; e < VE; ++e) g[e] = (ok >> (c * VE + e) & 1u) ? z[e] + add[c * VE + e] : ninf;
                     }
-                    if (!out) continue;
-                    if (scaled) {
-                        unpack<T, VE>(in[k], z);
-#pragma unroll
-                        for (int e = 0; e < VE; ++e)
-                            if ((hit & ok) >> e & 1u) g[e] *= z[e] > 0.0f ? inv_rho : rho;
-                    }
-                } else {
-                    unpack<T, VE>(in[k], z);
-                    if (scaled) {
-#pragma unroll
-                        for (int e = 0; e < VE; ++e)
-                            if (hit >> e & 1u) z[e] *= z[e] > 0.0f ? inv_rho : rho;
-                    }
-#pragma unroll
-                    for (int e = 0; e < VE; ++e) g[e] = (ok >> e & 1u) ? z[e] + add[e] : ninf;
+                    store_raw<T, VE>(out + base + o, pack<T, VE>(g));
                 }
-                store_raw<T, VE>(out + base + (t + k) * pitch + at, pack<T, VE>(g));
-            }
-        }
     }
-    if (!a.cu && out)   // padding rows of the padded layout are zeros
-        for (int t = t_stop; t < tb; ++t) store_raw<T, VE>(out + base + t * pitch + at, zero);
-    if (GRAD && a.part) {
-        float *p = a.part + (static_cast<int64_t>(n) * a.chunks + chunk) * plane + at;
 #pragma unroll
-        for (int e = 0; e < VE; ++e) p[e] = db[e];
+    for (int c = 0; c < NV; ++c) {
+        if (at[c] >= plane) continue;
+        if (!STEP && !packed && out)   // padding rows of the padded layout are zeros
+            for (int t = t_stop[c]; t < tb; ++t) store_raw<T, VE>(out + base + t * pitch + at[c], zero);
+        if (GRAD && a.part) {
+            constexpr int W = VE < 4 ? VE : 4;
+            float *p = a.part + (n * a.chunks + chunk) * plane + at[c];
+#pragma unroll
+            for (int e = 0; e < VE; e += W) store_raw<float, W>(p + e, pack<float, W>(db + (GRAD ? c * VE + e : 0)));
+        }
     }
 }
 
-// bias gradient: out[o][c] = sum over p of part[o][p][c], a block for every 32 columns of every o
+// Bias gradient out of the blocks' partial sums, out[o][c] = sum over p of part[o][p][c].  With few partials a thread
+// adds up four columns by itself; with many a block has 32 columns and one of `segments` runs of partials, and
+// where there is more than one run a second launch adds up the runs.
 template <typename T>
-__global__ void __launch_bounds__(1024) k_adjust_reduce(const ReduceArgs a) {
+__global__ void __launch_bounds__(256) k_adjust_reduce_few(const ReduceArgs a, int64_t outer) {
+    pdl_wait();
+    pdl_trigger();
+    if (a.C % 4 == 0) {
+        const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+        if (i >= outer * a.C) return;
+        const int64_t o = i / a.C;
+        const float *p = a.part + o * (a.P - 1) * a.C + i;
+        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+        for (int k = 0; k < static_cast<int>(a.P); ++k) {
+            const float4 v = *reinterpret_cast<const float4 *>(p + k * a.C);
+            x[0] += v.x;
+            x[1] += v.y;
+            x[2] += v.z;
+            x[3] += v.w;
+        }
+        if (a.out_f32)
+            store_raw<float, 4>(static_cast<float *>(a.out) + i, pack<float, 4>(x));
+        else
+            store_raw<T, 4>(static_cast<T *>(a.out) + i, pack<T, 4>(x));
+    } else {
+        const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+        if (i >= outer * a.C) return;
+        const float *p = a.part + i / a.C * (a.P - 1) * a.C + i;
+        float x = 0.0f;
+#pragma unroll 8
+        for (int k = 0; k < static_cast<int>(a.P); ++k) x += p[k * a.C];
+        if (a.out_f32)
+            static_cast<float *>(a.out)[i] = x;
+        else
+            static_cast<T *>(a.out)[i] = from_float<T>(x);
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(1024) k_adjust_reduce(const ReduceArgs a, int segments, float *runs) {
     __shared__ float sm[32][33];
     pdl_wait();
+    pdl_trigger();
     const unsigned col_blocks = static_cast<unsigned>((a.C + 31) / 32);
-    reduce_columns<T, 32, 32>(a, blockIdx.x % col_blocks, blockIdx.x / col_blocks, sm);
+    const unsigned col = blockIdx.x % col_blocks, q = blockIdx.x / col_blocks;
+    const int seg = q % segments;
+    const int64_t o = q / segments, len = (a.P + segments - 1) / segments, first = min(seg * len, a.P);
+    ReduceArgs r = a;
+    r.part = a.part + (o * a.P + first) * a.C;
+    r.P = min(len, a.P - first);
+    if (segments > 1) {
+        r.out = runs + (o * segments + seg) * a.C;
+        r.out_f32 = 1;
+    } else {
+        r.out = a.out_f32 ? static_cast<void *>(static_cast<float *>(a.out) + o * a.C) : static_cast<void *>(static_cast<T *>(a.out) + o * a.C);
+    }
+    reduce_columns<T, 32, 32>(r, col, 0, sm);
 }
 
 }  // namespace ctct

@@ -213,20 +213,49 @@ AdjGeom adj_geom(int64_t N, int64_t T, int64_t U1, int64_t V) {
     g.chunks = T > 0 ? ceil_div(T, g.tspan) : 1;
     return g;
 }
+// Partial sums of the bias gradient: `outer` results of `P` partials of `C` columns.  Up to ADJ_FEW partials a thread
+// adds them up (at N = 16, T = 512, U1 V = 132096 the blocks of 32 x 32 threads took 320 us for 8 partials
+// a column, most of their threads idle); beyond, runs of about 512 so that one shared row of V columns still
+// fills the GPU (8320 partials of 512 columns in one run: 52 us on 16 blocks).
+constexpr int64_t ADJ_FEW = 16;
+struct AdjReduce {
+    int64_t outer, P, C, segments;
+    size_t parts, total;   // bytes: partial sums, and with the runs behind them
+};
+AdjReduce adj_reduce(int64_t N, int64_t T, int64_t U1, int64_t V, int bias_kind) {
+    const int64_t chunks = adj_geom(N, T, U1, V).chunks;
+    AdjReduce r;
+    r.outer = bias_kind == 1 ? 1 : N;
+    r.P = bias_kind == 1 ? N * chunks * U1 : bias_kind == 2 ? chunks * U1 : chunks;
+    r.C = bias_kind == 3 ? U1 * V : V;
+    r.segments = ceil_div(r.P, 512);
+    if (r.segments > 32) r.segments = 32;
+    if (r.segments < 1) r.segments = 1;
+    r.parts = align256(static_cast<size_t>(N) * chunks * U1 * V * 4);
+    r.total = r.parts + (r.segments > 1 ? align256(static_cast<size_t>(r.outer) * r.segments * r.C * 4) : 0);
+    return r;
+}
 bool adj_dims_ok(int64_t N, int64_t T, int64_t U1, int64_t V) {
     return N >= 0 && N <= kMaxGrid && T >= 0 && U1 >= 1 && V >= 1 && U1 < (int64_t(1) << 31) && V < (int64_t(1) << 31) &&
            T < (int64_t(1) << 31) && U1 * V < (int64_t(1) << 31) - 4096;
 }
-template <typename T, int VE, bool GRAD>
-int adj_launch(AdjArgs &a, int64_t N, bool tail, cudaStream_t st) {
+template <typename T, bool GRAD>
+int adj_launch(AdjArgs &a, bool vec, int64_t N, bool tail, cudaStream_t st) {
+    constexpr int VE = 16 / static_cast<int>(sizeof(T));
     const int64_t plane = static_cast<int64_t>(a.U1) * a.V;
-    const int64_t chunks_of_plane = ceil_div(plane, VE);
-    const int threads = chunks_of_plane < ADJ_THREADS ? static_cast<int>(ceil_div(chunks_of_plane, 32) * 32) : ADJ_THREADS;
-    a.tiles = static_cast<int>(ceil_div(chunks_of_plane, threads));
+    // one row per n: a decoder's step
+    const bool step = a.T == 1 && a.U1 == 1 && !a.cu && !a.lx && !a.ly && (!a.tokens || a.tokens_len);
+    const int64_t per = step ? (vec ? 2 * VE : 8) : vec ? VE : 4;   // elements of a thread
+    const int64_t need = ceil_div(plane, per);
+    const int threads = need < ADJ_THREADS ? static_cast<int>(ceil_div(need, 32) * 32) : ADJ_THREADS;
+    a.tiles = static_cast<int>(ceil_div(plane, threads * per));
     const int64_t blocks = N * a.tiles * a.chunks;
     if (blocks > kMaxGrid - 64) return CTCT_ERR_UNSUPPORTED;
     a.main_blocks = static_cast<unsigned>(blocks);
-    launch_pdl(k_adjust<T, VE, GRAD>, dim3(static_cast<unsigned>(blocks + (tail ? 16 : 0))), dim3(threads), 0, st, a);
+    auto kernel = step ? (vec ? k_adjust<T, VE, 2, GRAD, true> : k_adjust<T, 1, 8, GRAD, true>)
+                       : (vec ? k_adjust<T, VE, 1, GRAD, false> : k_adjust<T, 1, 4, GRAD, false>);
+    launch_pdl(kernel, dim3(static_cast<unsigned>(blocks + (tail ? 16 : 0))),
+               dim3(threads), 0, st, a);
     return check_launch("adjust");
 }
 
@@ -421,9 +450,9 @@ int ctct_b200_joint_norm_backward(const void *dy, const void *f, int64_t f_sn, i
     });
 }
 
-size_t ctct_b200_adjust_workspace_bytes(int64_t N, int64_t T, int64_t U1, int64_t V) {
-    if (!adj_dims_ok(N, T, U1, V)) return 0;
-    return align256(static_cast<size_t>(N) * adj_geom(N, T, U1, V).chunks * U1 * V * 4);
+size_t ctct_b200_adjust_workspace_bytes(int64_t N, int64_t T, int64_t U1, int64_t V, int bias_kind) {
+    if (!adj_dims_ok(N, T, U1, V) || bias_kind < 1 || bias_kind > 3) return 0;
+    return adj_reduce(N, T, U1, V, bias_kind).total;
 }
 
 namespace {
@@ -450,7 +479,9 @@ int adj_fill(const AdjCall &c, int dtype, AdjArgs *a) {
     if (c.tokens_pitch < 0 || (c.tokens && !c.tokens_len && c.tokens_pitch < c.U1 - 1)) return CTCT_ERR_ARG;
     if (!c.rho_n && !(c.rho > 0.0f)) return CTCT_ERR_ARG;
     const int64_t words = ceil_div(c.V, 32);
-    a->tokens = c.tokens_pitch > 0 ? c.tokens : nullptr;
+    // histories that change nothing are not counted
+    const bool counts = c.rho_n || c.rho != 1.0f || c.presence_n || c.presence != 0.0f || c.frequency_n || c.frequency != 0.0f;
+    a->tokens = c.tokens_pitch > 0 && counts ? c.tokens : nullptr;
     a->tokens_len = c.tokens_len;
     a->L = c.tokens_pitch;
     a->lx = c.lx;
@@ -505,10 +536,7 @@ int ctct_b200_adjust_forward(const void *logits, int64_t row_stride, int dtype, 
     const int64_t E = 16 / static_cast<int64_t>(es);
     const bool vec = V % E == 0 && row_stride % E == 0 && aligned(logits, 16) && aligned(out, 16) && aligned(bias, 16);
     return with_type(dtype, [&](auto t) {
-        using T_ = decltype(t);
-        constexpr int VE = 16 / static_cast<int>(sizeof(T_));
-        const cudaStream_t st = static_cast<cudaStream_t>(stream);
-        return vec ? adj_launch<T_, VE, false>(a, N, packed_rows >= 0, st) : adj_launch<T_, 1, false>(a, N, packed_rows >= 0, st);
+        return adj_launch<decltype(t), false>(a, vec, N, packed_rows >= 0, static_cast<cudaStream_t>(stream));
     });
 }
 
@@ -523,47 +551,43 @@ int ctct_b200_adjust_backward(const void *dy, const void *logits, int64_t row_st
     if (int rc = adj_fill(c, dtype, &a)) return rc;
     if ((dbias && bias_kind == 0) || row_stride < 0 || (row_stride > 0 && (T != 1 || U1 != 1 || packed_rows >= 0))) return CTCT_ERR_ARG;
     const int64_t rows = packed_rows >= 0 ? packed_rows : N * T * U1;
-    const size_t need = static_cast<size_t>(N) * a.chunks * U1 * V * 4;
+    const AdjReduce red = adj_reduce(N, T, U1, V, bias_kind);
+    // one partial sum, laid out like the result: the blocks write the result themselves
+    const bool direct = dbias && red.P == 1 && a.bias_f32;
     if (rows > 0 && (!dy || (dx && a.tokens && (repetition_n || repetition != 1.0f) && !logits))) return CTCT_ERR_ARG;
-    if (rows > 0 && dbias && (!workspace || !aligned(workspace, 256) || workspace_bytes < need)) return CTCT_ERR_WORKSPACE;
+    if (rows > 0 && dbias && !direct && (!workspace || !aligned(workspace, 256) || workspace_bytes < red.total)) return CTCT_ERR_WORKSPACE;
     a.x = logits;
     a.x_sn = row_stride;
     a.dy = dy;
     a.y = dx;
-    a.part = dbias ? static_cast<float *>(workspace) : nullptr;
+    a.part = dbias ? static_cast<float *>(direct ? dbias : workspace) : nullptr;
     const size_t es = esize(dtype);
     const int64_t E = 16 / static_cast<int64_t>(es);
-    const bool vec = V % E == 0 && row_stride % E == 0 && aligned(logits, 16) && aligned(dx, 16) && aligned(dy, 16);
+    const bool vec = V % E == 0 && row_stride % E == 0 && aligned(logits, 16) && aligned(dx, 16) && aligned(dy, 16) && aligned(a.part, 16);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     return with_type(dtype, [&](auto t) -> int {
         using T_ = decltype(t);
-        constexpr int VE = 16 / static_cast<int>(sizeof(T_));
-        if (rows > 0 && N * T > 0) {
-            const bool tail = packed_rows >= 0 && dx;
-            const int rc = vec ? adj_launch<T_, VE, true>(a, N, tail, st) : adj_launch<T_, 1, true>(a, N, tail, st);
-            if (rc) return rc;
-        }
-        if (!dbias) return CTCT_OK;
-        const int64_t P = rows > 0 && N * T > 0 ? a.chunks : 0;  // no row: zeros
-        ReduceArgs r{static_cast<const float *>(workspace), dbias, a.bias_f32, 0, 0};
-        int64_t outer = 1;
-        if (bias_kind == 1) {
-            r.P = N * P * U1;
-            r.C = V;
-        } else if (bias_kind == 2) {
-            outer = N;
-            r.P = P * U1;
-            r.C = V;
-        } else {
-            outer = N;
-            r.P = P;
-            r.C = U1 * V;
-        }
-        if (outer == 0) return CTCT_OK;
-        const int64_t col_blocks = ceil_div(r.C, 32);
-        if (outer * col_blocks > kMaxGrid) return CTCT_ERR_UNSUPPORTED;
-        launch_pdl(k_adjust_reduce<T_>, dim3(static_cast<unsigned>(outer * col_blocks)), dim3(1024), 0, st, r);
-        return check_launch("adjust_reduce");
+        const bool some = rows > 0 && N * T > 0;
+        if (some)
+            if (int rc = adj_launch<T_, true>(a, vec, N, packed_rows >= 0 && dx, st)) return rc;
+        if (!dbias || (direct && some) || red.outer == 0) return CTCT_OK;
+        float *parts = static_cast<float *>(workspace), *runs = some ? parts + red.parts / 4 : nullptr;
+        ReduceArgs r{parts, dbias, a.bias_f32, some ? red.P : 0, red.C};   // no row: zeros
+        auto few = [&](const ReduceArgs &r) {
+            const int64_t blocks = ceil_div(red.outer * r.C, r.C % 4 == 0 ? 1024 : 256);
+            if (blocks > kMaxGrid) return static_cast<int>(CTCT_ERR_UNSUPPORTED);
+            launch_pdl(k_adjust_reduce_few<T_>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, r, red.outer);
+            return check_launch("adjust_reduce");
+        };
+        if (r.P <= ADJ_FEW) return few(r);
+        const int64_t blocks = red.outer * red.segments * ceil_div(r.C, 32);
+        if (blocks > kMaxGrid) return CTCT_ERR_UNSUPPORTED;
+        launch_pdl(k_adjust_reduce<T_>, dim3(static_cast<unsigned>(blocks)), dim3(1024), 0, st, r, static_cast<int>(red.segments), runs);
+        int rc = check_launch("adjust_reduce");
+        if (rc || red.segments == 1) return rc;
+        r.part = runs;
+        r.P = red.segments;
+        return few(r);
     });
 }
 
