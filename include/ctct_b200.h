@@ -466,7 +466,7 @@ int ctct_b200_layer_norm_backward(const void *dy, int64_t dy_stride, const void 
  */
 #define CTCT_MAX_JOINT_H 8192
 size_t ctct_b200_joint_norm_saved_bytes(int64_t N, int64_t T, int64_t U1, int64_t packed_rows, int want_grad);
-size_t ctct_b200_joint_norm_workspace_bytes(int64_t N, int64_t T, int64_t U1, int64_t H);
+size_t ctct_b200_joint_norm_workspace_bytes(int64_t N, int64_t T, int64_t U1, int64_t H, int dtype);
 int ctct_b200_joint_norm_forward(const void *f, int64_t f_sn, int64_t f_st, const void *g, int64_t g_sn, int64_t g_su,
                                  int dtype, const int32_t *lx, const int32_t *ly, int64_t N, int64_t T, int64_t U1,
                                  int64_t H, int64_t packed_rows, const void *weight, const void *bias, int param_f32,

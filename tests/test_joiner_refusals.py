@@ -62,8 +62,8 @@ def test_joint_norm_entry_points_refuse_bad_arguments(lib):
     assert lib.ctct_b200_joint_norm_saved_bytes(2, 3, 4, -1, 0) == 0   # nothing is kept without a gradient
     assert lib.ctct_b200_joint_norm_saved_bytes(2, 3, 4, 10, 0) >= 24
     assert lib.ctct_b200_joint_norm_saved_bytes(2, 3, 4, -1, 1) >= 4 * (6 + 8 + 24)
-    assert lib.ctct_b200_joint_norm_workspace_bytes(2, 3, 4, 8193) == 0
-    assert lib.ctct_b200_joint_norm_workspace_bytes(2, 3, 4, 8192) > 0
+    assert lib.ctct_b200_joint_norm_workspace_bytes(2, 3, 4, 8193, 0) == 0
+    assert lib.ctct_b200_joint_norm_workspace_bytes(2, 3, 4, 8192, 0) > 0
 
     def fwd(f=p, g=p, dtype=0, lx=p, ly=p, N=2, T=3, U1=4, H=8, rows=-1, y=p, grad=0, saved=None, nbytes=0):
         return lib.ctct_b200_joint_norm_forward(f, T * H, H, g, U1 * H, H, dtype, lx, ly, N, T, U1, H, rows, None, None, 1, 1e-5, y,

@@ -74,7 +74,7 @@ SIGNATURES = {
     "ctct_b200_layer_norm_backward": (_int, [_vp, _i64, _vp, _i64, _int, _i64, _i64, _vp, _int, _vp, _vp, _vp, _vp, _vp, _sz,
                                              _vp]),
     "ctct_b200_joint_norm_saved_bytes": (_sz, [_i64, _i64, _i64, _i64, _int]),
-    "ctct_b200_joint_norm_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),
+    "ctct_b200_joint_norm_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _int]),
     "ctct_b200_joint_norm_forward": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _int, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
                                             _vp, _vp, _int, C.c_float, _vp, _int, _vp, _sz, _vp]),
     "ctct_b200_joint_norm_backward": (_int, [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _int, _vp, _vp, _i64, _i64, _i64, _i64,
@@ -151,6 +151,21 @@ class on_device:
         if self.prev != self.index:
             torch.cuda.set_device(self.prev)
         return False
+
+
+def enter_device(device) -> int:
+    """Makes `device` the current CUDA device; the one to go back to with `leave_device`, or -1.  The pair is
+    `on_device` without its object, for calls that are over in a few microseconds."""
+    now = torch._C._cuda_getDevice()
+    if now == device.index:
+        return -1
+    torch.cuda.set_device(device.index)
+    return now
+
+
+def leave_device(previous: int) -> None:
+    if previous >= 0:
+        torch.cuda.set_device(previous)
 
 
 def workspace(N: int, T: int, U1: int, want_grad: bool, device) -> torch.Tensor:

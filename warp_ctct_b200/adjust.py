@@ -14,6 +14,8 @@ history of a row is its context's labels.  Gradients flow to the logits and to t
 """
 from __future__ import annotations
 
+from collections import namedtuple
+from math import inf
 from typing import Optional, Union
 
 import torch
@@ -34,18 +36,11 @@ def pack_token_mask(mask: T) -> T:
     return torch.where(packed >= 1 << 31, packed - (1 << 32), packed).to(torch.int32)
 
 
-class _Call:
-    """The arguments of one adjustment, checked: what the C entry points of both directions take."""
-
-    __slots__ = ("N", "T", "U1", "V", "rows", "row_stride", "tokens", "pitch", "lengths", "lx", "ly", "cu", "bias_kind", "bias_dtype",
-                 "allowed", "mask_kind", "scalars", "tensors")
-
-
 def _penalty(name: str, value: Union[float, T], N: int, device, positive: bool):
     """(scalar, tensor or None) of a penalty given as a number or as (N,) float32."""
     if not isinstance(value, torch.Tensor):
         value = float(value)
-        if not (value > 0.0 if positive else value == value) or value in (float("inf"), float("-inf")):
+        if not (0.0 < value < inf if positive else -inf < value < inf):
             raise RuntimeError(f"{name} must be a finite number{' above 0' if positive else ''}, not {value}")
         return value, None
     if value.dim() != 1 or value.size(0) != N:
@@ -54,7 +49,7 @@ def _penalty(name: str, value: Union[float, T], N: int, device, positive: bool):
         raise RuntimeError(f"{name} must be float32 on {device}")
     if value.requires_grad:
         raise RuntimeError(f"{name} is not differentiated: detach it")
-    return 1.0, value.contiguous()
+    return 1.0, value if value.is_contiguous() else value.contiguous()
 
 
 def _kind(name: str, t: Optional[T], N: int, U1: int, last: int, step: bool, device) -> int:
@@ -63,53 +58,67 @@ def _kind(name: str, t: Optional[T], N: int, U1: int, last: int, step: bool, dev
         return 0
     if t.device != device:
         raise RuntimeError(f"{name} must be on {device}, not on {t.device}")
-    for kind, shape in ((1, (last,)), (2, (N, last)), (3, (N, U1, last))):
-        if tuple(t.shape) == shape and not (step and kind == 3):
-            return kind
+    kind = t.dim()
+    if 1 <= kind <= (2 if step else 3) and t.size(-1) == last and (kind == 1 or t.size(0) == N) and (kind < 3 or t.size(1) == U1):
+        return kind
     per_context = "" if step else f" or ({N}, {U1}, {last})"
     raise RuntimeError(f"{name} must have shape ({last},), ({N}, {last}){per_context}, not {tuple(t.shape)}")
 
 
-def _prepare(logits: T, N: int, Tm: int, U1: int, rows: int, row_stride: int, tokens: Optional[T], pitch: int, lengths: Optional[T],
-             lx: Optional[T], ly: Optional[T], bias: Optional[T], allowed: Optional[T], repetition, presence, frequency, step: bool):
-    dev = logits.device
-    V = logits.size(-1)
-    if V < 1:
-        raise RuntimeError("logits must have at least one token")
-    c = _Call()
-    c.N, c.T, c.U1, c.V, c.rows, c.row_stride = N, Tm, U1, V, rows, row_stride
-    c.tokens, c.pitch, c.lengths, c.lx, c.ly, c.cu = tokens, pitch, lengths, lx, ly, None
-    c.bias_kind = _kind("bias", bias, N, U1, V, step, dev)
-    c.bias_dtype = None
-    if bias is not None:
-        if bias.dtype != logits.dtype and bias.dtype != torch.float32:
-            raise RuntimeError(f"bias must be float32 or of the logits' type {logits.dtype}, not {bias.dtype}")
-        c.bias_dtype = bias.dtype
-    c.mask_kind = _kind("allowed", allowed, N, U1, (V + 31) // 32, step, dev)
-    if allowed is not None and allowed.dtype != torch.int32:
-        raise RuntimeError("allowed must be int32 words (pack_token_mask)")
-    c.allowed = None if allowed is None else allowed.contiguous()
-    r, rn = _penalty("repetition_penalty", repetition, N, dev, True)
-    p, pn = _penalty("presence_penalty", presence, N, dev, False)
-    q, qn = _penalty("frequency_penalty", frequency, N, dev, False)
-    c.scalars, c.tensors = (r, p, q), (rn, pn, qn)
-    return c
+# What both directions of a call have in common.  shape: (N, T, U1, V, rows), rows < 0 for the padded layout and the
+# step; bias: (kind, 1 if float32); scalars, tensors: the penalties as `_penalty` gives them.
+_Call = namedtuple("_Call", "shape row_stride code tokens pitch lengths lx ly bias allowed mask_kind scalars tensors")
 
 
-def _forward(c: _Call, logits: T, bias: Optional[T]) -> T:
+def _forward(c: _Call, logits: T, bias: Optional[T]):
+    N, Tm, U1, V, rows = c.shape
     dev = logits.device
-    with _lib.on_device(dev):
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-        if c.rows >= 0:
-            c.cu = torch.empty((c.N + 1,), dtype=torch.int64, device=dev)
+    prev = _lib.enter_device(dev)
+    try:
+        out = torch.empty_like(logits) if c.row_stride == 0 else logits.new_empty(logits.shape)
+        cu = torch.empty((N + 1,), dtype=torch.int64, device=dev) if rows >= 0 else None
+        tokens, lengths, lx, ly, allowed = c.tokens, c.lengths, c.lx, c.ly, c.allowed
         rn, pn, qn = c.tensors
         rc = _lib.lib().ctct_b200_adjust_forward(
-            logits.data_ptr(), c.row_stride, _lib.dtype_code(logits.dtype), _lib.ptr(c.tokens), c.pitch, _lib.ptr(c.lengths),
-            _lib.ptr(c.lx), _lib.ptr(c.ly), c.N, c.T, c.U1, c.V, c.rows, _lib.ptr(c.cu), _lib.ptr(bias), c.bias_kind,
-            int(c.bias_dtype == torch.float32), _lib.ptr(c.allowed), c.mask_kind, *c.scalars, _lib.ptr(rn), _lib.ptr(pn),
-            _lib.ptr(qn), out.data_ptr(), _lib.raw_stream(dev))
-    _lib.check(rc, "ctct_b200_adjust_forward")
-    return out
+            logits.data_ptr(), c.row_stride, c.code, None if tokens is None else tokens.data_ptr(), c.pitch,
+            None if lengths is None else lengths.data_ptr(), None if lx is None else lx.data_ptr(),
+            None if ly is None else ly.data_ptr(), N, Tm, U1, V, rows, None if cu is None else cu.data_ptr(),
+            None if bias is None else bias.data_ptr(), *c.bias, None if allowed is None else allowed.data_ptr(), c.mask_kind,
+            *c.scalars, None if rn is None else rn.data_ptr(), None if pn is None else pn.data_ptr(),
+            None if qn is None else qn.data_ptr(), out.data_ptr(), _lib.raw_stream(dev))
+    finally:
+        _lib.leave_device(prev)
+    if rc:
+        _lib.check(rc, "ctct_b200_adjust_forward")
+    return out, cu
+
+
+def _backward(ctx, dy: T):
+    logits, tokens, lengths, lx, ly, cu, allowed, rn = ctx.saved_tensors
+    shape, row_stride, code, pitch, bias_meta, mask_kind, repetition = ctx.call
+    out_shape, dtype, dev, bias_shape, bias_dtype = ctx.like
+    N, Tm, U1, V, rows = shape
+    lib = _lib.lib()
+    if not dy.is_contiguous():
+        dy = dy.contiguous()
+    need_x, need_b = ctx.needs_input_grad[:2]
+    prev = _lib.enter_device(dev)
+    try:
+        dx = torch.empty(out_shape, dtype=dtype, device=dev) if need_x else None
+        db = torch.empty(bias_shape, dtype=bias_dtype, device=dev) if need_b else None
+        ws, nbytes = None, 0
+        if need_b:
+            nbytes = lib.ctct_b200_adjust_workspace_bytes(N, Tm, U1, V, bias_meta[0])
+            ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+        rc = lib.ctct_b200_adjust_backward(
+            dy.data_ptr(), _lib.ptr(logits), row_stride, code, _lib.ptr(tokens), pitch, _lib.ptr(lengths), _lib.ptr(lx),
+            _lib.ptr(ly), N, Tm, U1, V, rows, _lib.ptr(cu), *bias_meta, _lib.ptr(allowed), mask_kind, repetition, _lib.ptr(rn),
+            _lib.ptr(dx), _lib.ptr(db), _lib.ptr(ws), nbytes, _lib.raw_stream(dev))
+    finally:
+        _lib.leave_device(prev)
+    if rc:
+        _lib.check(rc, "ctct_b200_adjust_backward")
+    return dx, db, None
 
 
 class AdjustLogits(torch.autograd.Function):
@@ -117,53 +126,63 @@ class AdjustLogits(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits: T, bias: Optional[T], c: _Call):
-        out = _forward(c, logits, bias)
+        out, cu = _forward(c, logits, bias)
         scaled = c.tokens is not None and (c.tensors[0] is not None or c.scalars[0] != 1.0)
         # tensors that a caller could change in between go through save_for_backward, which notices
-        ctx.save_for_backward(logits if scaled else None, c.tokens, c.lengths, c.lx, c.ly, c.cu, c.allowed, c.tensors[0])
-        ctx.c, ctx.like = c, (logits.shape, logits.dtype, logits.device, None if bias is None else bias.shape)
-        c.tokens = c.lengths = c.lx = c.ly = c.cu = c.allowed = c.tensors = None
+        ctx.save_for_backward(logits if scaled else None, c.tokens, c.lengths, c.lx, c.ly, cu, c.allowed, c.tensors[0])
+        ctx.call = (c.shape, c.row_stride, c.code, c.pitch, c.bias, c.mask_kind, c.scalars[0])
+        ctx.like = (logits.shape, logits.dtype, logits.device, *((None, None) if bias is None else (bias.shape, bias.dtype)))
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy: T):
-        logits, tokens, lengths, lx, ly, cu, allowed, rn = ctx.saved_tensors
-        c, (shape, dtype, dev, bias_shape) = ctx.c, ctx.like
-        lib = _lib.lib()
-        dy = dy.contiguous()
-        need_x, need_b = ctx.needs_input_grad[:2]
-        with _lib.on_device(dev):
-            dx = torch.empty(shape, dtype=dtype, device=dev) if need_x else None
-            db = torch.empty(bias_shape, dtype=c.bias_dtype, device=dev) if need_b else None
-            ws, nbytes = None, 0
-            if need_b:
-                nbytes = lib.ctct_b200_adjust_workspace_bytes(c.N, c.T, c.U1, c.V, c.bias_kind)
-                ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
-            rc = lib.ctct_b200_adjust_backward(
-                dy.data_ptr(), _lib.ptr(logits), c.row_stride, _lib.dtype_code(dtype), _lib.ptr(tokens), c.pitch,
-                _lib.ptr(lengths), _lib.ptr(lx), _lib.ptr(ly), c.N, c.T, c.U1, c.V, c.rows, _lib.ptr(cu), c.bias_kind,
-                int(c.bias_dtype == torch.float32), _lib.ptr(allowed), c.mask_kind, c.scalars[0], _lib.ptr(rn), _lib.ptr(dx),
-                _lib.ptr(db), _lib.ptr(ws), nbytes, _lib.raw_stream(dev))
-        _lib.check(rc, "ctct_b200_adjust_backward")
-        return dx, db, None
+        # a graph of the gradient is only asked for with create_graph: the guard against a second
+        # differentiation costs nothing otherwise
+        return _backward_once(ctx, dy) if torch.is_grad_enabled() else _backward(ctx, dy)
 
 
-def _apply(c: _Call, logits: T, bias: Optional[T]) -> T:
-    if bias is not None and not bias.is_contiguous():
-        bias = bias.contiguous()
+_backward_once = once_differentiable(_backward)
+
+
+def _apply(logits: T, N: int, Tm: int, U1: int, rows: int, row_stride: int, tokens: Optional[T], pitch: int, lengths: Optional[T],
+           lx: Optional[T], ly: Optional[T], bias: Optional[T], allowed: Optional[T], repetition, presence, frequency,
+           step: bool) -> T:
+    dev, dtype = logits.device, logits.dtype
+    V = logits.size(-1)
+    if V < 1:
+        raise RuntimeError("logits must have at least one token")
+    bias_kind = _kind("bias", bias, N, U1, V, step, dev)
+    bias_f32 = 0
+    if bias_kind:
+        bias_f32 = int(bias.dtype == torch.float32)
+        if not bias_f32 and bias.dtype != dtype:
+            raise RuntimeError(f"bias must be float32 or of the logits' type {dtype}, not {bias.dtype}")
+        if not bias.is_contiguous():
+            bias = bias.contiguous()
+    mask_kind = _kind("allowed", allowed, N, U1, (V + 31) // 32, step, dev)
+    if mask_kind:
+        if allowed.dtype != torch.int32:
+            raise RuntimeError("allowed must be int32 words (pack_token_mask)")
+        if not allowed.is_contiguous():
+            allowed = allowed.contiguous()
+    r, rn = _penalty("repetition_penalty", repetition, N, dev, True)
+    p, pn = _penalty("presence_penalty", presence, N, dev, False)
+    q, qn = _penalty("frequency_penalty", frequency, N, dev, False)
+    c = _Call((N, Tm, U1, V, rows), row_stride, _lib.dtype_code(dtype), tokens, pitch, lengths, lx, ly, (bias_kind, bias_f32), allowed,
+              mask_kind, (r, p, q), (rn, pn, qn))
     if torch.is_grad_enabled() and (logits.requires_grad or (bias is not None and bias.requires_grad)):
         return AdjustLogits.apply(logits, bias, c)
-    return _forward(c, logits, bias)
+    return _forward(c, logits, bias)[0]
 
 
 def _int_on(name: str, t: T, device) -> T:
-    from . import _as_int
     if t.device != device:
         raise RuntimeError(f"{name} must be on {device}, not on {t.device}")
+    if t.dtype == torch.int32:
+        return t if t.is_contiguous() else t.contiguous()
     if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
         raise RuntimeError(f"{name} must hold integers, not {t.dtype}")
-    return _as_int(t)
+    return t.to(torch.int32).contiguous()
 
 
 def adjust_logits(logits: T, tokens: Optional[T] = None, tokens_lengths: Optional[T] = None, bias: Optional[T] = None,
@@ -204,9 +223,8 @@ def adjust_logits(logits: T, tokens: Optional[T] = None, tokens_lengths: Optiona
         raise RuntimeError("tokens_lengths without tokens")
     else:
         L = 0
-    c = _prepare(logits, R, 1, 1, -1, 0 if logits.is_contiguous() else logits.stride(0), tokens, L, tokens_lengths, None, None, bias,
-                 allowed, repetition_penalty, presence_penalty, frequency_penalty, True)
-    return _apply(c, logits, bias)
+    return _apply(logits, R, 1, 1, -1, 0 if logits.is_contiguous() else logits.stride(0), tokens, L, tokens_lengths, None, None, bias,
+                  allowed, repetition_penalty, presence_penalty, frequency_penalty, True)
 
 
 def _joint_args(logits: T, labels: T, frames_lengths: Optional[T], labels_lengths: Optional[T]):
@@ -244,9 +262,8 @@ def adjust_joint_logits(logits: T, labels: T, frames_lengths: Optional[T] = None
         raise RuntimeError("logits must have shape (N, T, U, V), labels (N, U - 1)")
     logits = logits.contiguous()
     N, Tm, U1, _ = logits.shape
-    c = _prepare(logits, N, Tm, U1, -1, 0, labels, U1 - 1, None, lx, ly, bias, allowed, repetition_penalty, presence_penalty,
-                 frequency_penalty, False)
-    return _apply(c, logits, bias)
+    return _apply(logits, N, Tm, U1, -1, 0, labels, U1 - 1, None, lx, ly, bias, allowed, repetition_penalty, presence_penalty,
+                  frequency_penalty, False)
 
 
 def adjust_joint_logits_packed(logits: T, labels: T, frames_lengths: T, labels_lengths: T, max_frames: Optional[int] = None,
@@ -266,6 +283,5 @@ def adjust_joint_logits_packed(logits: T, labels: T, frames_lengths: T, labels_l
         raise RuntimeError("max_frames must not be negative")
     logits = logits.contiguous()
     U1 = labels.size(1) + 1
-    c = _prepare(logits, labels.size(0), int(max_frames), U1, logits.size(0), 0, labels, U1 - 1, None, lx, ly, bias, allowed,
-                 repetition_penalty, presence_penalty, frequency_penalty, False)
-    return _apply(c, logits, bias)
+    return _apply(logits, labels.size(0), int(max_frames), U1, logits.size(0), 0, labels, U1 - 1, None, lx, ly, bias, allowed,
+                  repetition_penalty, presence_penalty, frequency_penalty, False)

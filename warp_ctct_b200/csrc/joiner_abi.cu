@@ -11,9 +11,6 @@
 
 using namespace ctct;
 
-#ifndef JG_REGS
-#define JG_REGS 168
-#endif
 namespace {
 
 size_t esize(int dtype) { return dtype == CTCT_F32 ? 4 : 2; }
@@ -45,7 +42,13 @@ struct LnGeom {
     int threads;
     int64_t grid;
 };
-LnGeom ln_geom(int64_t rows, int64_t H, int dtype) {
+#ifndef LN_FT
+#define LN_FT 1024
+#endif
+#ifndef LN_BT
+#define LN_BT 512
+#endif
+LnGeom ln_geom(int64_t rows, int64_t H, int dtype, int per_sm) {
     LnGeom g;
     g.P = ln_elems(H, dtype);
     g.is_long = H > static_cast<int64_t>(g.P) * LN_WIDE_THREADS;
@@ -53,7 +56,7 @@ LnGeom ln_geom(int64_t rows, int64_t H, int dtype) {
     g.threads = g.is_long ? LN_WIDE_THREADS : g.wide ? static_cast<int>(ceil_div(H, 32 * g.P)) * 32 : 32 * LN_WARPS;
     // resident blocks: 512 threads' worth per SM
     const int64_t blocks = g.wide ? rows : ceil_div(rows, LN_WARPS);
-    const int64_t most = static_cast<int64_t>(kSms) * (512 / g.threads > 0 ? 512 / g.threads : 1);
+    const int64_t most = static_cast<int64_t>(kSms) * (per_sm / g.threads > 0 ? per_sm / g.threads : 1);
     g.grid = blocks < most ? blocks : most;
     return g;
 }
@@ -102,9 +105,6 @@ struct JnGeom {
 };
 // Forward: columns per thread and frames per block: 8 x 4 up to 2048 columns (16-byte accesses of 16-bit types, at
 // most 256 threads), 32 x 1 beyond, where a row's sums need all threads of a block (a path for completeness).
-#ifndef JG_ACC
-#define JG_ACC 26
-#endif
 constexpr int JN_THREADS = 256;
 void jn_split(int64_t N, int64_t T, int64_t U1, int64_t tspan, int64_t uspan, JnGeom *g) {
     g->ublocks = static_cast<int>(ceil_div(U1, uspan));
@@ -124,21 +124,31 @@ bool jn_forward_geom(int64_t N, int64_t T, int64_t U1, int64_t H, JnGeom *g) {
     jn_split(N, T, U1, TF, uspan, g);
     return g->blocks <= kMaxGrid - 64;
 }
-// Backward: a thread has 8 columns, a block all of a row.  A block's contexts are as many as its share of shared
-// memory holds (36 KB: six blocks of 64 threads on an SM at H = 512, as many as registers allow), its frames as many
-// as leave a dozen blocks for every SM, since utterances are of different lengths.
-bool jn_grad_geom(int64_t N, int64_t T, int64_t U1, int64_t H, JnGeom *g) {
+// Backward: a thread has 8 columns, a block all of a row.  Registers say how many blocks an SM holds, their share of
+// shared memory then how many contexts a block takes beside its ring.  As many blocks as the GPU holds at a
+// time, or a multiple of it, each with an equal share of the cells, at most JG_BLOCKS of them.
+bool jn_grad_geom(int64_t N, int64_t T, int64_t U1, int64_t H, int dtype, JnGeom *g) {
     if (H < 1 || H > CTCT_MAX_JOINT_H) return false;
     g->P = JG_P;
     g->threads = static_cast<int>(ceil_div(H, 32 * JG_P) * 32);
-    const int64_t per_context = static_cast<int64_t>(g->threads) * JG_P * 4;
-    int64_t uspan = (JG_ACC * 1024) / per_context;
-    uspan = uspan < 1 ? 1 : uspan > U1 ? U1 : uspan;
-    int64_t tspan = 16 * JG_TF;
-    while (tspan > JG_TF && N * ceil_div(T, tspan) * ceil_div(U1, uspan) < 12 * kSms) tspan /= 2;
-    while (uspan > 1 && N * ceil_div(T, tspan) * ceil_div(U1, uspan) < kSms) uspan = (uspan + 1) / 2;
-    jn_split(N, T, U1, tspan, uspan, g);
-    g->smem = jg_smem_bytes(g->threads, g->tspan, g->uspan);
+    const bool wide = g->threads > JG_MAX_THREADS;
+    const int64_t regs = wide ? JG_WIDE_REGS : JG_REGS;
+    int64_t resident = 65536 / (regs * g->threads);
+    resident = resident < 1 ? 1 : resident > 12 ? 12 : resident;
+    const int64_t ring = wide ? 0 : static_cast<int64_t>(jg_ring_bytes(g->threads, static_cast<int>(esize(dtype))));
+    // of an SM's 228 KB a block pays 1 KB to the system, and 512 bytes of static memory and padding
+    const int64_t share = 228 * 1024 / resident - 1024 - 512 - ring;
+    const int64_t fixed = static_cast<int64_t>(jg_smem_bytes(g->threads, 0)), per = static_cast<int64_t>(jg_smem_bytes(g->threads, 1)) - fixed;
+    int64_t uspan = (share - fixed) / per;
+    uspan = uspan < 1 ? 1 : uspan > 32 ? 32 : uspan;
+    if (uspan > U1) uspan = U1;
+    const int64_t cells_t = ceil_div(T, JG_TF), slots = kSms * resident;
+    while (uspan > 1 && N * cells_t * ceil_div(U1, uspan) < kSms) uspan = (uspan + 1) / 2;   // small: use all SMs
+    jn_split(N, T, U1, JG_TF, uspan, g);
+    const int64_t cells = g->blocks;
+    g->blocks = slots * ceil_div(cells, slots * JG_BLOCKS);
+    if (g->blocks > cells) g->blocks = cells;
+    g->smem = jg_smem_bytes(g->threads, g->uspan);
     return g->blocks <= kMaxGrid;
 }
 bool jn_dims_ok(int64_t N, int64_t T, int64_t U1, int64_t H) {
@@ -163,14 +173,15 @@ JnSaved jn_saved(int64_t N, int64_t T, int64_t U1, int64_t packed_rows, int want
     return s;
 }
 struct JnWs {
-    size_t f, g, w, total;
+    size_t f, g, w, cells, total;
 };
 JnWs jn_ws(int64_t N, int64_t T, int64_t U1, int64_t H, const JnGeom &g) {
     JnWs w;
     w.f = 0;
     w.g = align256(static_cast<size_t>(N) * g.ublocks * T * H * 4);
-    w.w = align256(w.g + static_cast<size_t>(N) * g.tblocks * U1 * H * 4);
-    w.total = align256(w.w + 2 * static_cast<size_t>(g.blocks) * H * 4);
+    w.w = align256(w.g + static_cast<size_t>(g.blocks + N * g.ublocks) * g.uspan * H * 4);
+    w.cells = align256(w.w + 2 * static_cast<size_t>(g.blocks) * H * 4);
+    w.total = align256(w.cells + static_cast<size_t>(N + 1) * 8);
     return w;
 }
 JnShape jn_shape(const int32_t *lx, const int32_t *ly, const int64_t *cu, int64_t packed_rows, int64_t N, int64_t T, int64_t U1,
@@ -265,7 +276,7 @@ extern "C" {
 
 size_t ctct_b200_layer_norm_workspace_bytes(int64_t rows, int64_t H, int dtype) {
     if (rows < 0 || H < 1 || H >= (int64_t(1) << 31) || !dtype_ok(dtype)) return 0;
-    return align256(2 * static_cast<size_t>(ln_geom(rows, H, dtype).grid) * H * 4);
+    return align256(2 * static_cast<size_t>(ln_geom(rows, H, dtype, LN_BT).grid) * H * 4);
 }
 
 int ctct_b200_layer_norm_forward(const void *x, int64_t x_stride, int dtype, int64_t rows, int64_t H, const void *weight,
@@ -278,7 +289,7 @@ int ctct_b200_layer_norm_forward(const void *x, int64_t x_stride, int dtype, int
                      aligned(bias, 16);
     LnArgs a{x, x_stride, weight, bias, param_f32 || dtype == CTCT_F32, eps, y, reinterpret_cast<float2 *>(stats), rows,
              static_cast<int>(H)};
-    const LnGeom g = ln_geom(rows, H, dtype);
+    const LnGeom g = ln_geom(rows, H, dtype, LN_FT);
     return with_type(dtype, [&](auto t) {
         ln_dispatch<decltype(t)>(g, vec, a, static_cast<cudaStream_t>(stream));
         return check_launch("layer_norm");
@@ -291,7 +302,7 @@ int ctct_b200_layer_norm_backward(const void *dy, int64_t dy_stride, const void 
     if (rows < 0 || H < 1 || H >= (int64_t(1) << 31) || !dtype_ok(dtype) || (rows > 0 && (!dy || !x || !stats))) return CTCT_ERR_ARG;
     const bool params = dweight || dbias;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    LnGeom g = ln_geom(rows, H, dtype);
+    const LnGeom g = ln_geom(rows, H, dtype, LN_BT);
     if (params && rows > 0 && (!workspace || !aligned(workspace, 256) || workspace_bytes < 2 * static_cast<size_t>(g.grid) * H * 4))
         return CTCT_ERR_WORKSPACE;
     const size_t es = esize(dtype);
@@ -319,9 +330,9 @@ size_t ctct_b200_joint_norm_saved_bytes(int64_t N, int64_t T, int64_t U1, int64_
     return jn_saved(N, T, U1, packed_rows, want_grad).total;
 }
 
-size_t ctct_b200_joint_norm_workspace_bytes(int64_t N, int64_t T, int64_t U1, int64_t H) {
+size_t ctct_b200_joint_norm_workspace_bytes(int64_t N, int64_t T, int64_t U1, int64_t H, int dtype) {
     JnGeom g;
-    if (!jn_dims_ok(N, T, U1, H) || !jn_grad_geom(N, T, U1, H, &g)) return 0;
+    if (!jn_dims_ok(N, T, U1, H) || !dtype_ok(dtype) || !jn_grad_geom(N, T, U1, H, dtype, &g)) return 0;
     return jn_ws(N, T, U1, H, g).total;
 }
 
@@ -381,7 +392,7 @@ int ctct_b200_joint_norm_backward(const void *dy, const void *f, int64_t f_sn, i
     if (!jn_dims_ok(N, T, U1, H) || !dtype_ok(dtype)) return CTCT_ERR_ARG;
     if (packed && (!lx || !ly) && N > 0) return CTCT_ERR_ARG;
     JnGeom geo;
-    if (!jn_grad_geom(N, T, U1, H, &geo)) return CTCT_ERR_UNSUPPORTED;
+    if (!jn_grad_geom(N, T, U1, H, dtype, &geo)) return CTCT_ERR_UNSUPPORTED;
     const JnSaved sv = jn_saved(N, T, U1, packed_rows, 1);
     const JnWs ws = jn_ws(N, T, U1, H, geo);
     if (rows > 0 && (!dy || (N > 0 && T > 0 && (!f || !g)))) return CTCT_ERR_ARG;
@@ -410,8 +421,10 @@ int ctct_b200_joint_norm_backward(const void *dy, const void *f, int64_t f_sn, i
     a.part_f = reinterpret_cast<float *>(wb + ws.f);
     a.part_g = reinterpret_cast<float *>(wb + ws.g);
     a.part_w = reinterpret_cast<float *>(wb + ws.w);
+    a.cells = reinterpret_cast<int64_t *>(wb + ws.cells);
     const bool some = rows > 0 && geo.blocks > 0;
     JnReduceArgs r;
+    r.cells = a.cells;
     r.s = a.s;
     r.part_f = a.part_f;
     r.part_g = a.part_g;
@@ -433,8 +446,8 @@ int ctct_b200_joint_norm_backward(const void *dy, const void *f, int64_t f_sn, i
         using E_ = decltype(t);
         constexpr int VE = sizeof(E_) == 4 ? 4 : 8;
         if (some) {
-            auto kernel = geo.threads <= JG_MAX_THREADS ? (vec ? k_joint_norm_grad<E_, VE, JG_REGS> : k_joint_norm_grad<E_, 1, 168>)
-                                                        : (vec ? k_joint_norm_grad<E_, VE, 64> : k_joint_norm_grad<E_, 1, 64>);
+            auto kernel = geo.threads <= JG_MAX_THREADS ? (vec ? k_joint_norm_grad<E_, VE, JG_REGS> : k_joint_norm_grad<E_, 1, JG_REGS>)
+                                                        : (vec ? k_joint_norm_grad<E_, VE, JG_WIDE_REGS> : k_joint_norm_grad<E_, 1, JG_WIDE_REGS>);
             // beyond 48 KB an attribute is needed; it belongs to the current device: set with the launch
             const size_t smem = align256(geo.smem) + (vec && geo.threads <= JG_MAX_THREADS ? jg_ring_bytes(geo.threads, sizeof(E_)) : 0);
             if (smem > 48 * 1024 &&

@@ -68,8 +68,9 @@ struct JnGradArgs {
     const void *dy;
     const float *fm, *gm, *rstd;
     float *part_f;       // [N][ublocks][T][H]: df
-    float *part_g;       // [N][tblocks][U1][H]: dg
+    float *part_g;       // [segment][uspan][H]: dg
     float *part_w;       // [2][gridDim.x][H]: dw, db
+    int64_t *cells;      // out: cells before utterance n (N + 1)
     int ring_offset;     // bytes of shared memory before the ring
 };
 
@@ -346,16 +347,27 @@ __global__ void __maxnreg__(128) k_joint_norm(const JnArgs a) {
 
 constexpr int JG_P = 8, JG_TF = 4;      // columns per thread, frames per block of registers
 constexpr int JG_MAX_THREADS = 256;
+constexpr int JG_REGS = 168, JG_WIDE_REGS = 64;   // registers per thread up to JG_MAX_THREADS, and of the wide kernels
 constexpr int JG_BATCH = 8;             // contexts whose g is on its way together behind the stream
-// Shared memory of a block (floats): B [uspan][P / 4][team][4], private to the threads; c1 and c2 [uspan][warps][2 * TF];
-// k1 and k2 of the present frames [uspan][2 * TF]; k2 of all frames, negative, each twice [tspan / TF][uspan][2 * TF]; sums
-// of k1 and of -k2 over the frames [uspan][2].
-#ifndef JG_STAGES
-#define JG_STAGES 2
-#endif
+constexpr int JG_BLOCKS = 16;           // most blocks of TF frames that a thread block takes
+constexpr int JG_STAGES = 2;            // of a thread's ring of rows of dy
+// Shared memory of a block (floats): B [uspan][P / 4][team][4] and dw [P / 2][team][2], private to the threads; c1 and c2
+// [uspan][warps][2 * TF];
+// k1 and k2 of the present frames [uspan][2 * TF]; r of the present frames [uspan][TF]; -k2 of all frames
+// [JG_BLOCKS][uspan][TF]; sums of k1 and of -k2 over the frames [uspan][2].
 inline size_t jg_ring_bytes(int threads, int esize) { return static_cast<size_t>(JG_STAGES) * JG_TF * JG_P * esize * threads; }
-inline size_t jg_smem_bytes(int threads, int tspan, int uspan) {
-    return 4 * static_cast<size_t>(uspan) * (threads * JG_P + threads / 32 * 2 * JG_TF + 2 * JG_TF + tspan / JG_TF * 2 * JG_TF + 2);
+inline size_t jg_smem_bytes(int threads, int uspan) {
+    return 4 * (static_cast<size_t>(uspan) * (threads * JG_P + threads / 32 * 2 * JG_TF + 3 * JG_TF + JG_BLOCKS * JG_TF + 2) + threads * JG_P);
+}
+
+// The work of the gradient launch: cells of TF frames x uspan contexts, utterance after utterance, range of contexts after
+// range of contexts, along the frames last.  Block i of G (at most W) takes cells [i W / G, (i + 1) W / G) of the W that hold
+// valid rows, so that blocks of ragged batches end together (fixed tiles of 16 frames: 160 us instead of 122 at 32x256x65x512
+// bf16).  A block's run inside one (utterance, range) is a segment; segments are numbered block + N-th (utterance, range),
+// which grows with every step along the runs, and each leaves one partial sum of dg.
+__device__ __forceinline__ int64_t jg_cells(const JnShape &s, int n) {
+    const int Tn = s.frames(n);
+    return static_cast<int64_t>((Tn + JG_TF - 1) / JG_TF) * ((s.contexts(n) + s.uspan - 1) / s.uspan);
 }
 
 // REGS: registers per thread; six blocks of 64 threads on an SM with 168
@@ -367,12 +379,13 @@ __global__ void __maxnreg__(REGS) k_joint_norm_grad(const JnGradArgs a) {
     pdl_trigger();
     const JnShape &s = a.s;
     const int tid = threadIdx.x, team = blockDim.x, lane = tid & 31, warps = team >> 5;
-    float *const cs = acc_b + static_cast<size_t>(s.uspan) * P * team;
+    float *const dws = acc_b + static_cast<size_t>(s.uspan) * P * team;
+    float *const cs = dws + P * team;
     float *const ks = cs + s.uspan * warps * 2 * TF;
-    float *const k2s = ks + s.uspan * 2 * TF;
-    float *const sums = k2s + (s.tspan / TF) * s.uspan * 2 * TF;   // sums of k1 and of -k2 over the frames, per context
+    float *const rs = ks + s.uspan * 2 * TF;
+    float *const k2s = rs + s.uspan * TF;
+    float *const sums = k2s + JG_BLOCKS * s.uspan * TF;
     uint4 *const ring = reinterpret_cast<uint4 *>(reinterpret_cast<char *>(acc_b) + a.ring_offset) + tid;
-    const unsigned tile = blockIdx.x;
     int col[NV], at[NV];
     bool in[NV];
 #pragma unroll
@@ -381,30 +394,84 @@ __global__ void __maxnreg__(REGS) k_joint_norm_grad(const JnGradArgs a) {
         in[i] = col[i] < s.H;
         at[i] = in[i] ? col[i] : 0;
     }
-    const int ub = tile % s.ublocks, q_ = tile / s.ublocks;
-    const int tb = q_ % s.tblocks, n = q_ / s.tblocks;
-    const int Tn = s.frames(n), Un = s.contexts(n);
-    const int u0 = ub * s.uspan, ue = min(min(u0 + s.uspan, s.U1), Un);
-    const int ta = tb * s.tspan, te = min(min(ta + s.tspan, s.T), Tn);
-    const int64_t base = s.first_row(n);
-    const int pitch = s.row_pitch(Un);
-    const int64_t pitch_h = static_cast<int64_t>(pitch) * s.H;
+    // this block's cells: a scan of the utterances' (a thread has a run of them)
+    __shared__ int64_t scan[32];
+    // where the block stands: utterance, cells of it that lie behind, cells still to do.  Here, not in registers,
+    // since the loops below need all of those.
+    __shared__ int64_t at_cell;
+    __shared__ int at_n, left;
+    const int per = (s.N + team - 1) / team, n_lo = min(tid * per, s.N), n_hi = min(n_lo + per, s.N);
+    int64_t mine = 0;
+    for (int i = n_lo; i < n_hi; ++i) mine += jg_cells(s, i);
+    int64_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+    }
+    if (lane == 31) scan[tid >> 5] = upto;
+    __syncthreads();
+    int64_t before = upto - mine, W = 0;
+    for (int i = 0; i < warps; ++i) {
+        if (i < (tid >> 5)) before += scan[i];
+        W += scan[i];
+    }
+    if (blockIdx.x == 0) {
+        int64_t c = before;
+        for (int i = n_lo; i < n_hi; ++i) {
+            a.cells[i] = c;
+            c += jg_cells(s, i);
+        }
+        if (tid == 0) a.cells[s.N] = W;
+    }
+    const int64_t G = min(static_cast<int64_t>(gridDim.x), W);   // every block below G has a cell, so has every segment
+    const int64_t cell = blockIdx.x < G ? W * blockIdx.x / G : W;
+    if (tid == 0) left = blockIdx.x < G ? static_cast<int>(W * (blockIdx.x + 1) / G - cell) : 0;
+    if (before <= cell && cell < before + mine) {
+        int64_t c = before;
+        int i = n_lo;
+        for (;; ++i) {
+            const int64_t v = jg_cells(s, i);
+            if (cell < c + v) break;
+            c += v;
+        }
+        at_n = i;
+        at_cell = cell - c;
+    }
+    __syncthreads();
     const float inv_h = 1.0f / static_cast<float>(s.H);
     const F2 z2 = f2(0.0f, 0.0f);
-    F2 dw[Q], db[Q];
+    F2 db[Q], w[Q];
+    // dw is added to once per TF frames: it lives in shared memory, two columns at a time in the thread's own places
+    auto add_dw = [&](int i, const F2 &x, const F2 &y) {
+        F2 *to = reinterpret_cast<F2 *>(dws) + i * team + tid;
+        *to = fma2(x, y, *to);
+    };
 #pragma unroll
-    for (int i = 0; i < Q; ++i) dw[i] = db[i] = z2;
-    if (ta < te && u0 < ue) {
-        F2 w[Q];
-        {
-            float wv[P];
+    for (int i = 0; i < Q; ++i) {
+        db[i] = z2;
+        reinterpret_cast<F2 *>(dws)[i * team + tid] = z2;
+    }
+    {
+        float wv[P];
 #pragma unroll
-            for (int i = 0; i < P; ++i) wv[i] = in[i / VE] ? 1.0f : 0.0f;
+        for (int i = 0; i < P; ++i) wv[i] = in[i / VE] ? 1.0f : 0.0f;
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
-                if (in[i] && a.w) load_param<T, VE>(a.w, a.p_f32, col[i], wv + i * VE);
-            pair_up<P>(wv, w);
-        }
+        for (int i = 0; i < NV; ++i)
+            if (in[i] && a.w) load_param<T, VE>(a.w, a.p_f32, col[i], wv + i * VE);
+        pair_up<P>(wv, w);
+    }
+    while (left > 0) {
+        const int n = at_n;
+        const int Tn = s.frames(n), Un = s.contexts(n);
+        const int cells_t = (Tn + TF - 1) / TF;
+        const int ub = static_cast<int>(at_cell / cells_t), tb = static_cast<int>(at_cell - static_cast<int64_t>(ub) * cells_t);
+        const int run = min(cells_t - tb, left);
+        const int u0 = ub * s.uspan, ue = min(min(u0 + s.uspan, s.U1), Un);
+        const int ta = tb * TF, te = min(ta + run * TF, Tn);
+        const int64_t base = s.first_row(n);
+        const int pitch = s.row_pitch(Un);
+        const int64_t pitch_h = static_cast<int64_t>(pitch) * s.H;
         for (int i = 0; i < (ue - u0) * (P / 4); ++i)
             *reinterpret_cast<float4 *>(acc_b + (static_cast<size_t>(i) * team + tid) * 4) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         for (int u = tid; u < ue - u0; u += team) sums[2 * u] = 0.0f;
@@ -480,7 +547,7 @@ __global__ void __maxnreg__(REGS) k_joint_norm_grad(const JnGradArgs a) {
             // FULL: all frames and rows are there; threads without columns read column 0 with a weight of zero
             auto walk = [&](auto full_tag) {
                 constexpr bool FULL = decltype(full_tag)::value;
-                constexpr bool RING = FULL && VE * sizeof(T) == 16 && REGS > 64;   // 1024 threads leave no room for it
+                constexpr bool RING = FULL && VE * sizeof(T) == 16 && REGS > JG_WIDE_REGS;   // 1024 threads leave no room for it
                 Raw<T, VE> rd[RING ? 1 : TF][NV], rg[NV];
                 int p_slot = 0, c_slot = 0;
                 auto issue = [&](bool some) {
@@ -584,7 +651,7 @@ __global__ void __maxnreg__(REGS) k_joint_norm_grad(const JnGradArgs a) {
                     const float sum = warp_sums<2 * TF>(v);
                     if ((lane & 3) == 0) {
                         *my_c = sum;
-                        if (tid < 4 * TF) ks[(u - u0) * 2 * TF + kl] = r_mine;
+                        if (tid < 4 * TF) rs[(u - u0) * TF + kl] = r_mine;
                     }
                     my_c += warps * 2 * TF;
 #pragma unroll
@@ -604,7 +671,7 @@ __global__ void __maxnreg__(REGS) k_joint_norm_grad(const JnGradArgs a) {
             __syncthreads();
             for (int i = tid; i < (ue - u0) * TF; i += team) {
                 const int u = i / TF, k = i % TF;
-                const float r = ks[u * 2 * TF + k];   // left there by the stream; k1 takes its place
+                const float r = rs[i];   // left there by the stream
                 float c1 = 0.0f, c2 = 0.0f;
                 for (int p = 0; p < warps; ++p) {
                     const float *c = cs + (u * warps + p) * 2 * TF + k;
@@ -614,8 +681,7 @@ __global__ void __maxnreg__(REGS) k_joint_norm_grad(const JnGradArgs a) {
                 const float k1 = r * (c1 * inv_h), k2 = r * r * (r * (c2 * inv_h));
                 ks[u * 2 * TF + k] = k1;
                 ks[u * 2 * TF + TF + k] = k2;
-                float *twice = k2s + ((t0 - ta) / TF * s.uspan + u) * 2 * TF + 2 * k;
-                twice[0] = twice[1] = -k2;
+                k2s[((t0 - ta) / TF * s.uspan + u) * TF + k] = -k2;
             }
             __syncthreads();
             for (int u = tid; u < ue - u0; u += team) {
@@ -627,14 +693,16 @@ __global__ void __maxnreg__(REGS) k_joint_norm_grad(const JnGradArgs a) {
 #pragma unroll
             for (int k = 0; k < TF / 2; ++k) k1_sum[k] = k2_sum[k] = z2;
 #pragma unroll
-            for (int k = 0; k < TF; ++k)
+            for (int i = 0; i < Q; ++i) {
+                F2 sum = z2;
 #pragma unroll
-                for (int i = 0; i < Q; ++i) {
-                    dw[i] = fma2(f[k][i], A[k][i], dw[i]);
+                for (int k = 0; k < TF; ++k) {
+                    sum = fma2(f[k][i], A[k][i], sum);
                     A[k][i] = mul2(w[i], A[k][i]);
                 }
+                add_dw(i, sum, f2(1.0f, 1.0f));
+            }
             {
-                const float *twice = k2s + (t0 - ta) / TF * s.uspan * 2 * TF;
                 for_g([&](int u, const F2 (&gc)[Q]) {
                     const ulonglong2 p1 = *reinterpret_cast<const ulonglong2 *>(ks + u * 2 * TF);
                     const ulonglong2 p2 = *reinterpret_cast<const ulonglong2 *>(ks + u * 2 * TF + TF);
@@ -642,9 +710,12 @@ __global__ void __maxnreg__(REGS) k_joint_norm_grad(const JnGradArgs a) {
                     k1_sum[1] = add2(k1_sum[1], F2{p1.y});
                     k2_sum[0] = add2(k2_sum[0], F2{p2.x});
                     k2_sum[1] = add2(k2_sum[1], F2{p2.y});
+                    float k2[TF];
+                    split(F2{p2.x}, k2[0], k2[1]);
+                    split(F2{p2.y}, k2[2], k2[3]);
 #pragma unroll
                     for (int k = 0; k < TF; ++k) {
-                        const F2 m = *reinterpret_cast<const F2 *>(twice + u * 2 * TF + 2 * k);
+                        const F2 m = f2(-k2[k], -k2[k]);
 #pragma unroll
                         for (int i = 0; i < Q; ++i) A[k][i] = fma2(m, gc[i], A[k][i]);
                     }
@@ -677,7 +748,7 @@ __global__ void __maxnreg__(REGS) k_joint_norm_grad(const JnGradArgs a) {
             float t = 0.0f;
             for (int i = 0; i < blocks; ++i)
 #pragma unroll
-                for (int k = 0; k < TF; ++k) t += k2s[(i * s.uspan + u) * 2 * TF + 2 * k];
+                for (int k = 0; k < TF; ++k) t += k2s[(i * s.uspan + u) * TF + k];
             sums[2 * u + 1] = t;
         }
         __syncthreads();
@@ -702,7 +773,7 @@ __global__ void __maxnreg__(REGS) k_joint_norm_grad(const JnGradArgs a) {
             const F2 m1 = f2(-k1, -k1), m2 = f2(k2, k2);
 #pragma unroll
             for (int e = 0; e < Q; ++e) {
-                dw[e] = fma2(gc[e], B[e], dw[e]);
+                add_dw(e, gc[e], B[e]);
                 B[e] = fma2(w[e], B[e], fma2(m2, gc[e], m1));
             }
             store_b(u, B);
@@ -714,17 +785,19 @@ __global__ void __maxnreg__(REGS) k_joint_norm_grad(const JnGradArgs a) {
             for (int u = 0; u < ue - u0; ++u) {
                 F2 B[Q];
                 load_b(u, B);
-                const float *twice = k2s + (i * s.uspan + u) * 2 * TF;
+                float k2[TF];
+                unpack<float, 4>(*reinterpret_cast<const uint4 *>(k2s + (i * s.uspan + u) * TF), k2);
 #pragma unroll
                 for (int k = 0; k < TF; ++k) {
-                    const F2 m = *reinterpret_cast<const F2 *>(twice + 2 * k);
+                    const F2 m = f2(k2[k], k2[k]);
 #pragma unroll
                     for (int e = 0; e < Q; ++e) B[e] = fma2(m, f[k][e], B[e]);
                 }
                 if (i + 1 < blocks) {
                     store_b(u, B);
                 } else {
-                    float *out = a.part_g + ((static_cast<int64_t>(n) * s.tblocks + tb) * s.U1 + u0 + u) * s.H;
+                    const int64_t segment = static_cast<int64_t>(blockIdx.x) + static_cast<int64_t>(n) * s.ublocks + ub;
+                    float *out = a.part_g + (segment * s.uspan + u) * s.H;
                     float o[P];
                     unpair<P>(B, o);
 #pragma unroll
@@ -738,12 +811,27 @@ __global__ void __maxnreg__(REGS) k_joint_norm_grad(const JnGradArgs a) {
                 }
             }
         }
+        __syncthreads();   // all have read where the block stands, and the sums of this segment
+        if (tid == 0) {
+            left -= run;
+            int64_t c = at_cell + run;
+            int m = n;
+            if (left > 0)   // on to the next utterance with frames, if this one is done
+                while (c == jg_cells(s, m)) {
+                    ++m;
+                    c = 0;
+                }
+            at_n = m;
+            at_cell = c;
+        }
+        __syncthreads();
     }
-    float *pw = a.part_w + static_cast<int64_t>(tile) * s.H;
+    float *pw = a.part_w + static_cast<int64_t>(blockIdx.x) * s.H;
     float *pb = pw + static_cast<int64_t>(gridDim.x) * s.H;
     float ow[P], ob[P];
-    unpair<P>(dw, ow);
     unpair<P>(db, ob);
+#pragma unroll
+    for (int i = 0; i < Q; ++i) split(reinterpret_cast<const F2 *>(dws)[i * team + tid], ow[2 * i], ow[2 * i + 1]);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         if (in[i]) {
@@ -763,6 +851,7 @@ constexpr int JR_THREADS = 256, JR_COLS = 8;   // JR_COLS columns of dw or db a 
 struct JnReduceArgs {
     JnShape s;
     const float *part_f, *part_g, *part_w;
+    const int64_t *cells;
     void *df, *dg, *dw, *db;   // any of them nullptr
     int p_f32;
     int64_t parts_w;           // blocks of the gradient launch
@@ -784,16 +873,28 @@ __global__ void __launch_bounds__(JR_THREADS) k_joint_norm_reduce(const JnReduce
         return;
     }
     const bool is_f = blockIdx.x < a.w_blocks + a.f_blocks;
-    const int rows = is_f ? s.T : s.U1, parts_all = is_f ? s.ublocks : s.tblocks;
+    const int rows = is_f ? s.T : s.U1;
     void *out = is_f ? a.df : a.dg;
     const unsigned i = (blockIdx.x - a.w_blocks - (is_f ? 0 : a.f_blocks)) * (JR_THREADS / 32) + (threadIdx.x >> 5);
     if (!out || i >= static_cast<unsigned>(rows) * s.N) return;
     const int n = static_cast<int>(i / rows), r = static_cast<int>(i - static_cast<unsigned>(n) * rows);
     const int Tn = a.no_rows ? 0 : s.frames(n), Un = a.no_rows ? 0 : s.contexts(n);
-    const int along = is_f ? Un : Tn, span = is_f ? s.uspan : s.tspan;
-    const int parts = r < (is_f ? Tn : Un) ? (along + span - 1) / span : 0;
-    const int64_t plane = static_cast<int64_t>(rows) * s.H;
-    const float *p = (is_f ? a.part_f : a.part_g) + static_cast<int64_t>(n) * parts_all * plane + static_cast<int64_t>(r) * s.H;
+    int parts = 0;
+    int64_t plane = 0;     // from partial to partial
+    const float *p = nullptr;
+    if (is_f) {
+        plane = static_cast<int64_t>(s.T) * s.H;
+        p = a.part_f + (static_cast<int64_t>(n) * s.ublocks * s.T + r) * s.H;
+        if (r < Tn) parts = (Un + s.uspan - 1) / s.uspan;
+    } else if (r < Un && Tn > 0) {   // the segments of (n, r / uspan): one for every block that has cells of it
+        const int ub = r / s.uspan;
+        const int64_t W = a.cells[s.N], G = min(a.parts_w, W), cells_t = (Tn + JG_TF - 1) / JG_TF;
+        const int64_t c0 = a.cells[n] + ub * cells_t, c1 = c0 + cells_t - 1;
+        const int64_t b0 = ((c0 + 1) * G - 1) / W, b1 = ((c1 + 1) * G - 1) / W;   // the last block that begins at or before the cell
+        plane = static_cast<int64_t>(s.uspan) * s.H;
+        p = a.part_g + ((b0 + static_cast<int64_t>(n) * s.ublocks + ub) * s.uspan + (r - ub * s.uspan)) * s.H;
+        parts = static_cast<int>(b1 - b0 + 1);
+    }
     T *o = static_cast<T *>(out) + static_cast<int64_t>(i) * s.H;
     if (s.H % 4 == 0) {   // both buffers are whole vectors apart
         for (int col = (threadIdx.x & 31) * 4; col < s.H; col += 128) {

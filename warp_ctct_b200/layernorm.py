@@ -8,6 +8,7 @@ gradient once.  All sums are float32 and taken in a fixed order, so results are 
 """
 from __future__ import annotations
 
+from math import inf
 from typing import Optional
 
 import torch
@@ -21,25 +22,26 @@ T = torch.Tensor
 def _check_params(x: T, weight: Optional[T], bias: Optional[T], H: int) -> int:
     """Checks weight and bias against activations `x`; 1 if they are float32, 0 if they have x's type."""
     f32 = None
+    dtype, device = x.dtype, x.device
     for name, p in (("weight", weight), ("bias", bias)):
         if p is None:
             continue
         if p.dim() != 1 or p.size(0) != H:
             raise RuntimeError(f"{name} must have shape ({H},)")
-        if p.dtype != x.dtype and p.dtype != torch.float32:
-            raise RuntimeError(f"{name} must be float32 or of the activations' type {x.dtype}, not {p.dtype}")
-        if p.device != x.device:
-            raise RuntimeError(f"{name} must be on {x.device}, not on {p.device}")
-        is_f32 = p.dtype == torch.float32
-        if f32 is not None and f32 != is_f32:
+        pd = p.dtype
+        if pd != dtype and pd != torch.float32:
+            raise RuntimeError(f"{name} must be float32 or of the activations' type {dtype}, not {pd}")
+        if p.device != device:
+            raise RuntimeError(f"{name} must be on {device}, not on {p.device}")
+        if f32 is not None and f32 != (pd == torch.float32):
             raise RuntimeError("weight and bias must have the same type")
-        f32 = is_f32
-    return int(bool(f32))
+        f32 = pd == torch.float32
+    return 1 if f32 else 0
 
 
 def _check_eps(eps: float) -> float:
     eps = float(eps)
-    if not 0.0 <= eps < float("inf"):
+    if not 0.0 <= eps < inf:
         raise RuntimeError(f"eps must be a finite number that is not negative, not {eps}")
     return eps
 
@@ -48,11 +50,19 @@ def _dense(p: Optional[T]) -> Optional[T]:
     return p if p is None or p.is_contiguous() else p.contiguous()
 
 
+def _wants_grad(*tensors: Optional[T]) -> bool:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
 def _as_rows(x: T) -> T:
     """`x` as (rows, H) with adjacent elements in a row and one stride between rows; a copy if it has no such form."""
-    H = x.size(-1)
-    if x.dim() == 2 and (x.stride(1) == 1 or H == 1) and x.stride(0) >= 0:
+    if x.dim() == 2 and (x.stride(1) == 1 or x.size(1) == 1):
         return x
+    H = x.size(-1)
     if x.is_contiguous():
         return x.view(-1, H)
     if x.dim() == 2 or x.stride(-1) != 1:
@@ -66,14 +76,51 @@ def _as_rows(x: T) -> T:
 def _ln_forward(rows: T, weight: Optional[T], bias: Optional[T], p_f32: int, eps: float, want_grad: bool):
     R, H = rows.shape
     dev = rows.device
-    with _lib.on_device(dev):
-        y = torch.empty((R, H), dtype=rows.dtype, device=dev)
+    prev = _lib.enter_device(dev)
+    try:
+        y = torch.empty_like(rows) if rows.is_contiguous() else rows.new_empty((R, H))
         stats = torch.empty((R, 2), dtype=torch.float32, device=dev) if want_grad else None
         rc = _lib.lib().ctct_b200_layer_norm_forward(
-            rows.data_ptr(), rows.stride(0), _lib.dtype_code(rows.dtype), R, H, _lib.ptr(weight), _lib.ptr(bias), p_f32, eps,
-            y.data_ptr(), _lib.ptr(stats), _lib.raw_stream(dev))
-    _lib.check(rc, "ctct_b200_layer_norm_forward")
+            rows.data_ptr(), rows.stride(0), _lib.dtype_code(rows.dtype), R, H, None if weight is None else weight.data_ptr(),
+            None if bias is None else bias.data_ptr(), p_f32, eps, y.data_ptr(), stats.data_ptr() if want_grad else None,
+            _lib.raw_stream(dev))
+    finally:
+        _lib.leave_device(prev)
+    if rc:
+        _lib.check(rc, "ctct_b200_layer_norm_forward")
     return y, stats
+
+
+def _ln_backward(ctx, dy: T):
+    rows, weight, stats = ctx.saved_tensors
+    p_f32, bias_dtype = ctx.meta
+    R, H = rows.shape
+    dev = rows.device
+    lib = _lib.lib()
+    code = _lib.dtype_code(rows.dtype)
+    dy = _as_rows(dy)
+    need_x, need_w, need_b = ctx.needs_input_grad[:3]
+    prev = _lib.enter_device(dev)
+    try:
+        dx = dw = db = ws = None
+        nbytes = 0
+        if need_x:
+            dx = torch.empty_like(rows) if rows.is_contiguous() else rows.new_empty((R, H))
+        if need_w:
+            dw = torch.empty_like(weight)
+        if need_b:
+            db = torch.empty((H,), dtype=bias_dtype, device=dev)
+        if need_w or need_b:
+            nbytes = lib.ctct_b200_layer_norm_workspace_bytes(R, H, code)
+            ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+        rc = lib.ctct_b200_layer_norm_backward(
+            dy.data_ptr(), dy.stride(0), rows.data_ptr(), rows.stride(0), code, R, H, _lib.ptr(weight), p_f32, stats.data_ptr(),
+            _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db), _lib.ptr(ws), nbytes, _lib.raw_stream(dev))
+    finally:
+        _lib.leave_device(prev)
+    if rc:
+        _lib.check(rc, "ctct_b200_layer_norm_backward")
+    return dx, dw, db, None, None
 
 
 class LayerNorm(torch.autograd.Function):
@@ -87,29 +134,13 @@ class LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy: T):
-        rows, weight, stats = ctx.saved_tensors
-        p_f32, bias_dtype = ctx.meta
-        R, H = rows.shape
-        dev = rows.device
-        lib = _lib.lib()
-        code = _lib.dtype_code(rows.dtype)
-        dy = _as_rows(dy)
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        with _lib.on_device(dev):
-            dx = torch.empty((R, H), dtype=rows.dtype, device=dev) if need_x else None
-            dw = torch.empty((H,), dtype=weight.dtype, device=dev) if need_w else None
-            db = torch.empty((H,), dtype=bias_dtype, device=dev) if need_b else None
-            ws, nbytes = None, 0
-            if need_w or need_b:
-                nbytes = lib.ctct_b200_layer_norm_workspace_bytes(R, H, code)
-                ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
-            rc = lib.ctct_b200_layer_norm_backward(
-                dy.data_ptr(), dy.stride(0), rows.data_ptr(), rows.stride(0), code, R, H, _lib.ptr(weight), p_f32,
-                stats.data_ptr(), _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db), _lib.ptr(ws), nbytes, _lib.raw_stream(dev))
-        _lib.check(rc, "ctct_b200_layer_norm_backward")
-        return dx, dw, db, None, None
+        # a graph of the gradient is only asked for with create_graph: the guard against a second
+        # differentiation costs nothing otherwise
+        return _ln_backward_once(ctx, dy) if torch.is_grad_enabled() else _ln_backward(ctx, dy)
+
+
+_ln_backward_once = once_differentiable(_ln_backward)
 
 
 def layer_norm(x: T, weight: Optional[T] = None, bias: Optional[T] = None, eps: float = 1e-5) -> T:
@@ -125,17 +156,17 @@ def layer_norm(x: T, weight: Optional[T] = None, bias: Optional[T] = None, eps: 
     if not x.is_cuda:
         raise RuntimeError("x must be located in the CUDA")
     _lib.dtype_code(x.dtype)
-    if x.dim() < 1 or x.size(-1) < 1:
+    dims = x.dim()
+    if dims < 1 or x.size(-1) < 1:
         raise RuntimeError("x must have at least one dimension, with at least one element")
     p_f32 = _check_params(x, weight, bias, x.size(-1))
     eps = _check_eps(eps)
     rows, weight, bias = _as_rows(x), _dense(weight), _dense(bias)
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
+    if _wants_grad(x, weight, bias):
         y = LayerNorm.apply(rows, weight, bias, p_f32, eps)
     else:
         y, _ = _ln_forward(rows, weight, bias, p_f32, eps, False)
-    return y if x.dim() == 2 else y.view(x.shape)
+    return y if dims == 2 else y.view(x.shape)
 
 
 def _joint_forward(f: T, g: T, lx: Optional[T], ly: Optional[T], weight: Optional[T], bias: Optional[T], p_f32: int, eps: float,
@@ -145,18 +176,54 @@ def _joint_forward(f: T, g: T, lx: Optional[T], ly: Optional[T], weight: Optiona
     U1 = g.size(1)
     dev = f.device
     lib = _lib.lib()
-    with _lib.on_device(dev):
-        y = torch.empty((rows, H) if rows >= 0 else (N, Tm, U1, H), dtype=f.dtype, device=dev)
-        saved, nbytes = None, 0
+    prev = _lib.enter_device(dev)
+    try:
+        y = f.new_empty((rows, H) if rows >= 0 else (N, Tm, U1, H))
+        saved, saved_ptr, nbytes = None, None, 0
         if want_grad or rows >= 0:
             nbytes = lib.ctct_b200_joint_norm_saved_bytes(N, Tm, U1, rows, int(want_grad))
             saved = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+            saved_ptr = saved.data_ptr()
         rc = lib.ctct_b200_joint_norm_forward(
             f.data_ptr(), f.stride(0), f.stride(1), g.data_ptr(), g.stride(0), g.stride(1), _lib.dtype_code(f.dtype),
-            _lib.ptr(lx), _lib.ptr(ly), N, Tm, U1, H, rows, _lib.ptr(weight), _lib.ptr(bias), p_f32, eps, y.data_ptr(),
-            int(want_grad), _lib.ptr(saved), nbytes, _lib.raw_stream(dev))
-    _lib.check(rc, "ctct_b200_joint_norm_forward")
+            None if lx is None else lx.data_ptr(), None if ly is None else ly.data_ptr(), N, Tm, U1, H, rows,
+            None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(), p_f32, eps, y.data_ptr(),
+            want_grad, saved_ptr, nbytes, _lib.raw_stream(dev))
+    finally:
+        _lib.leave_device(prev)
+    if rc:
+        _lib.check(rc, "ctct_b200_joint_norm_forward")
     return y, saved
+
+
+def _joint_backward(ctx, dy: T):
+    f, g, weight, lx, ly, saved = ctx.saved_tensors
+    p_f32, rows, bias_dtype = ctx.meta
+    N, Tm, H = f.shape
+    U1 = g.size(1)
+    dev = f.device
+    lib = _lib.lib()
+    code = _lib.dtype_code(f.dtype)
+    if not dy.is_contiguous():
+        dy = dy.contiguous()
+    need_f, need_g, need_w, need_b = ctx.needs_input_grad[:4]
+    prev = _lib.enter_device(dev)
+    try:
+        df = f.new_empty((N, Tm, H)) if need_f else None
+        dg = f.new_empty((N, U1, H)) if need_g else None
+        dw = torch.empty_like(weight) if need_w else None
+        db = torch.empty((H,), dtype=bias_dtype, device=dev) if need_b else None
+        nbytes = lib.ctct_b200_joint_norm_workspace_bytes(N, Tm, U1, H, code)
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+        rc = lib.ctct_b200_joint_norm_backward(
+            dy.data_ptr(), f.data_ptr(), f.stride(0), f.stride(1), g.data_ptr(), g.stride(0), g.stride(1), code,
+            _lib.ptr(lx), _lib.ptr(ly), N, Tm, U1, H, rows, _lib.ptr(weight), p_f32, saved.data_ptr(), saved.numel(),
+            _lib.ptr(df), _lib.ptr(dg), _lib.ptr(dw), _lib.ptr(db), ws.data_ptr(), nbytes, _lib.raw_stream(dev))
+    finally:
+        _lib.leave_device(prev)
+    if rc:
+        _lib.check(rc, "ctct_b200_joint_norm_backward")
+    return df, dg, dw, db, None, None, None, None, None
 
 
 class JointLayerNorm(torch.autograd.Function):
@@ -171,49 +238,36 @@ class JointLayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy: T):
-        f, g, weight, lx, ly, saved = ctx.saved_tensors
-        p_f32, rows, bias_dtype = ctx.meta
-        N, Tm, H = f.shape
-        U1 = g.size(1)
-        dev = f.device
-        lib = _lib.lib()
-        dy = dy.contiguous()
-        need_f, need_g, need_w, need_b = ctx.needs_input_grad[:4]
-        with _lib.on_device(dev):
-            df = torch.empty((N, Tm, H), dtype=f.dtype, device=dev) if need_f else None
-            dg = torch.empty((N, U1, H), dtype=f.dtype, device=dev) if need_g else None
-            dw = torch.empty((H,), dtype=weight.dtype, device=dev) if need_w else None
-            db = torch.empty((H,), dtype=bias_dtype, device=dev) if need_b else None
-            nbytes = lib.ctct_b200_joint_norm_workspace_bytes(N, Tm, U1, H)
-            ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
-            rc = lib.ctct_b200_joint_norm_backward(
-                dy.data_ptr(), f.data_ptr(), f.stride(0), f.stride(1), g.data_ptr(), g.stride(0), g.stride(1),
-                _lib.dtype_code(f.dtype), _lib.ptr(lx), _lib.ptr(ly), N, Tm, U1, H, rows, _lib.ptr(weight), p_f32,
-                saved.data_ptr(), saved.numel(), _lib.ptr(df), _lib.ptr(dg), _lib.ptr(dw), _lib.ptr(db), ws.data_ptr(), nbytes,
-                _lib.raw_stream(dev))
-        _lib.check(rc, "ctct_b200_joint_norm_backward")
-        return df, dg, dw, db, None, None, None, None, None
+        return _joint_backward_once(ctx, dy) if torch.is_grad_enabled() else _joint_backward(ctx, dy)
+
+
+_joint_backward_once = once_differentiable(_joint_backward)
 
 
 def _joint(f: T, g: T, lx: Optional[T], ly: Optional[T], weight: Optional[T], bias: Optional[T], eps: float, rows: int) -> T:
     from . import _as_int
-    for name, t in (("f", f), ("g", g)):
-        if not t.is_cuda:
-            raise RuntimeError(f"{name} must be located in the CUDA")
+    if not f.is_cuda:
+        raise RuntimeError("f must be located in the CUDA")
+    if not g.is_cuda:
+        raise RuntimeError("g must be located in the CUDA")
     _lib.dtype_code(f.dtype)
-    if f.dim() != 3 or g.dim() != 3 or f.size(0) != g.size(0) or f.size(2) != g.size(2):
+    if f.dim() != 3 or g.dim() != 3:
+        raise RuntimeError("f and g must have shapes (N, T, H) and (N, U, H)")
+    N, _, H = f.shape
+    Ng, U1, Hg = g.shape
+    if N != Ng or H != Hg:
         raise RuntimeError("f and g must have shapes (N, T, H) and (N, U, H)")
     if g.dtype != f.dtype or g.device != f.device:
         raise RuntimeError("f and g must have the same type and device")
-    N, _, H = f.shape
-    if H < 1 or g.size(1) < 1:
+    if H < 1 or U1 < 1:
         raise RuntimeError("f and g must have at least one element per row, g at least one context")
     for name, t in (("frames_lengths", lx), ("labels_lengths", ly)):
-        if t is not None and (t.dim() != 1 or t.size(0) != N):
+        if t is None:
+            continue
+        if t.dim() != 1 or t.size(0) != N:
             raise RuntimeError(f"{name} must have shape ({N},)")
-        if t is not None and t.device != f.device:
+        if t.device != f.device:
             raise RuntimeError(f"{name} must be on {f.device}, not on {t.device}")
     p_f32 = _check_params(f, weight, bias, H)
     eps = _check_eps(eps)
@@ -224,8 +278,7 @@ def _joint(f: T, g: T, lx: Optional[T], ly: Optional[T], weight: Optional[T], bi
     weight, bias = _dense(weight), _dense(bias)
     lx = None if lx is None else _as_int(lx)
     ly = None if ly is None else _as_int(ly)
-    if torch.is_grad_enabled() and (f.requires_grad or g.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
+    if _wants_grad(f, g, weight, bias):
         return JointLayerNorm.apply(f, g, weight, bias, lx, ly, p_f32, eps, rows)
     return _joint_forward(f, g, lx, ly, weight, bias, p_f32, eps, rows, False)[0]
 
@@ -236,7 +289,7 @@ def joint_layer_norm(f: T, g: T, frames_lengths: Optional[T] = None, labels_leng
 
     Args:
         f: (N, T, H) encoder frames, g: (N, U, H) predictor states (U = max labels + 1), the same type: float32,
-            float16 or bfloat16.  Both may be slices or expanded, as long as a row's elements are adjacent.
+            float16 or bfloat16, H up to 8192.  Both may be slices or expanded, as long as a row's elements are adjacent.
         frames_lengths, labels_lengths: (N,) as in ``ctct_loss``; rows beyond them are zeros and take no
             part in any gradient.  None: all rows are valid.
         weight, bias, eps: as in ``layer_norm``.
