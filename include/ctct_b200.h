@@ -493,7 +493,7 @@ int ctct_b200_joint_norm_backward(const void *dy, const void *f, int64_t f_sn, i
  * bias), each may be NULL; `logits` is read only where a repeated token is scaled (NULL if repetition is 1 for all
  * rows); dy is not read in padding rows, masked places get zero.  workspace: ctct_b200_adjust_workspace_bytes, for dbias only.
  */
-size_t ctct_b200_adjust_workspace_bytes(int64_t N, int64_t T, int64_t U1, int64_t V, int bias_kind);
+size_t ctct_b200_adjust_workspace_bytes(int64_t N, int64_t T, int64_t U1, int64_t V, int dtype, int packed, int bias_kind);
 int ctct_b200_adjust_forward(const void *logits, int64_t row_stride, int dtype, const int32_t *tokens, int64_t tokens_pitch,
                              const int32_t *tokens_lengths, const int32_t *lx, const int32_t *ly, int64_t N, int64_t T,
                              int64_t U1, int64_t V, int64_t packed_rows, int64_t *cu_rows, const void *bias, int bias_kind,

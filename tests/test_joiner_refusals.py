@@ -87,8 +87,8 @@ def test_joint_norm_entry_points_refuse_bad_arguments(lib):
 
 def test_adjust_entry_points_refuse_bad_arguments(lib):
     p = 4096
-    assert lib.ctct_b200_adjust_workspace_bytes(2, 3, 4, 5, 2) >= 2 * 4 * 5 * 4
-    assert lib.ctct_b200_adjust_workspace_bytes(2, 3, 1 << 16, 1 << 16, 2) == 0   # a plane beyond 2^31 elements
+    assert lib.ctct_b200_adjust_workspace_bytes(2, 3, 4, 5, 0, 0, 2) >= 2 * 4 * 5 * 4
+    assert lib.ctct_b200_adjust_workspace_bytes(2, 3, 1 << 16, 1 << 16, 0, 0, 2) == 0   # a plane beyond 2^31 elements
 
     def fwd(x=p, stride=0, dtype=0, tok=p, pitch=3, lens=None, lx=None, ly=None, N=2, T=3, U1=4, V=8, rows=-1, cu=None, bias=None,
             bk=0, allowed=None, mk=0, rho=1.0, rho_n=None, out=p):

@@ -79,7 +79,7 @@ SIGNATURES = {
                                             _vp, _vp, _int, C.c_float, _vp, _int, _vp, _sz, _vp]),
     "ctct_b200_joint_norm_backward": (_int, [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _int, _vp, _vp, _i64, _i64, _i64, _i64,
                                              _i64, _vp, _int, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
-    "ctct_b200_adjust_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _int]),
+    "ctct_b200_adjust_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _int, _int, _int]),
     "ctct_b200_adjust_forward": (_int, [_vp, _i64, _int, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp,
                                         _int, _int, _vp, _int, C.c_float, C.c_float, C.c_float, _vp, _vp, _vp, _vp, _vp]),
     "ctct_b200_adjust_backward": (_int, [_vp, _vp, _i64, _int, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp,

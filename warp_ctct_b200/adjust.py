@@ -108,7 +108,7 @@ def _backward(ctx, dy: T):
         db = torch.empty(bias_shape, dtype=bias_dtype, device=dev) if need_b else None
         ws, nbytes = None, 0
         if need_b:
-            nbytes = lib.ctct_b200_adjust_workspace_bytes(N, Tm, U1, V, bias_meta[0])
+            nbytes = lib.ctct_b200_adjust_workspace_bytes(N, Tm, U1, V, code, int(rows >= 0), bias_meta[0])
             ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
         rc = lib.ctct_b200_adjust_backward(
             dy.data_ptr(), _lib.ptr(logits), row_stride, code, _lib.ptr(tokens), pitch, _lib.ptr(lengths), _lib.ptr(lx),

@@ -46,6 +46,7 @@ struct AdjArgs {
     float *part;               // backward: bias gradient of every block, [N][chunks][U1 * V], or nullptr
     int N, T, U1, V;
     int tspan, chunks;         // frames of a block, blocks along T
+    int classes;               // a block's frames are `classes` apart; `chunks` counts all classes of all runs
     int tiles;                 // blocks along the plane of U1 * V elements
     unsigned main_blocks;      // blocks beyond it clear packed rows behind the last utterance
 };
@@ -92,7 +93,10 @@ __global__ void __launch_bounds__(ADJ_THREADS, 4) k_adjust(const AdjArgs a) {
     const unsigned tile0 = tile * threads * NE, tile1 = min(tile0 + threads * NE, plane);
     const int u_first = STEP ? 0 : static_cast<int>(tile0 / V);
     const int u_last = STEP ? 0 : min(static_cast<int>((tile1 - 1) / V), Un - 1);
-    const int ta = STEP ? 0 : chunk * a.tspan, tb = STEP ? 1 : min(ta + a.tspan, a.T), te = max(ta, min(tb, Tn));
+    // the block's frames: ta, ta + ts, ... below tb
+    const int ts = STEP ? 1 : a.classes, run = STEP ? 0 : chunk / ts;
+    const int ta = STEP ? 0 : run * (a.tspan * ts) + (chunk - run * ts), tb = STEP ? 1 : min((run + 1) * (a.tspan * ts), a.T);
+    const int te = max(ta, min(tb, Tn));
     const bool work = u_first < Un && ta < te;
     // rows of this thread's elements: one every `pitch` elements
     const bool packed = !STEP && a.cu;
@@ -132,7 +136,7 @@ __global__ void __launch_bounds__(ADJ_THREADS, 4) k_adjust(const AdjArgs a) {
         for (int k = 0; k < UNROLL; ++k)
 #pragma unroll
             for (int c = 0; c < NV; ++c)
-                if (t + k < t_stop[c]) in[k][c] = load_once<T, VE>(from + (t + k) * pitch + at[c]);
+                if (t + k * ts < t_stop[c]) in[k][c] = load_once<T, VE>(from + (t + k * ts) * pitch + at[c]);
     };
     fetch(ta);
     const bool history = work && tok;
@@ -187,12 +191,12 @@ __global__ void __launch_bounds__(ADJ_THREADS, 4) k_adjust(const AdjArgs a) {
     int t_end = ta;
 #pragma unroll
     for (int c = 0; c < NV; ++c) t_end = max(t_end, t_stop[c]);
-    for (int t = ta; t < t_end; t += UNROLL) {
+    for (int t = ta; t < t_end; t += UNROLL * ts) {
         if (t > ta) fetch(t);
         if (STAGE && scaled && out) {   // a thread reads back what it copied itself: no barrier, and no registers
 #pragma unroll
             for (int k = 0; k < UNROLL; ++k)
-                if (t + k < t_stop[0]) cp_async16(xs + k * ADJ_THREADS + tid, x + (t + k) * pitch + at[0]);
+                if (t + k * ts < t_stop[0]) cp_async16(xs + k * ADJ_THREADS + tid, x + (t + k * ts) * pitch + at[0]);
             cp_async_commit();
             cp_async_wait<0>();
         }
@@ -200,8 +204,8 @@ __global__ void __launch_bounds__(ADJ_THREADS, 4) k_adjust(const AdjArgs a) {
         for (int k = 0; k < UNROLL; ++k)
 #pragma unroll
             for (int c = 0; c < NV; ++c)
-                if (t + k < t_stop[c]) {
-                    const int64_t o = (t + k) * pitch + at[c];
+                if (t + k * ts < t_stop[c]) {
+                    const int64_t o = (t + k * ts) * pitch + at[c];
                     float z[VE], g[VE];
                     unpack<T, VE>(in[k][c], z);
                     if (GRAD) {
@@ -238,13 +242,199 @@ __global__ void __launch_bounds__(ADJ_THREADS, 4) k_adjust(const AdjArgs a) {
     for (int c = 0; c < NV; ++c) {
         if (at[c] >= plane) continue;
         if (!STEP && !packed && out)   // padding rows of the padded layout are zeros
-            for (int t = t_stop[c]; t < tb; ++t) store_raw<T, VE>(out + base + t * pitch + at[c], zero);
+            for (int t = ta; t < tb; t += ts)
+                if (t >= t_stop[c]) store_raw<T, VE>(out + base + t * pitch + at[c], zero);
         if (GRAD && a.part) {
             constexpr int W = VE < 4 ? VE : 4;
             float *p = a.part + (n * a.chunks + chunk) * plane + at[c];
 #pragma unroll
             for (int e = 0; e < VE; e += W) store_raw<float, W>(p + e, pack<float, W>(db + (GRAD ? c * VE + e : 0)));
         }
+    }
+}
+
+// Rows that are no whole number of 16-byte vectors.  The plane of an utterance's frame is taken as one run of elements that
+// begins somewhere inside a vector: a thread owns one aligned vector of it, wherever that stands against rows.  The run
+// begins at the same place for frames that are a vector's number of elements apart, so a block's frames are that far
+// apart, and what is added to an element stays in its thread.  Only the two ends of a plane are accessed
+// element by element.  (With 2-byte accesses the f32-free step over 32x256x65x511 bf16 took 1146 us backward and 416
+// forward; whole rows of 512 take 261 and 193.)
+template <typename T, bool GRAD>
+__global__ void __launch_bounds__(ADJ_THREADS, 4) k_adjust_flat(const AdjArgs a) {
+    constexpr int VE = 16 / static_cast<int>(sizeof(T));
+    __shared__ __align__(16) int count[ADJ_THREADS * VE];
+    __shared__ uint4 xs[GRAD ? ADJ_UNROLL * ADJ_THREADS : 1];
+    pdl_wait();
+    pdl_trigger();
+    const int tid = threadIdx.x, threads = blockDim.x;
+    const Raw<T, VE> zero = Raw<T, VE>{};
+    T *out = static_cast<T *>(a.y);
+    if (blockIdx.x >= a.main_blocks) {
+        const int64_t end = a.packed_rows * a.V, step = static_cast<int64_t>(gridDim.x - a.main_blocks) * threads;
+        for (int64_t i = a.cu[a.N] * a.V + static_cast<int64_t>(blockIdx.x - a.main_blocks) * threads + tid; i < end; i += step)
+            out[i] = from_float<T>(0.0f);
+        return;
+    }
+    const unsigned q = blockIdx.x / static_cast<unsigned>(a.tiles), tile = blockIdx.x - q * a.tiles;
+    const int chunk = q % static_cast<unsigned>(a.chunks);
+    const int64_t n = q / static_cast<unsigned>(a.chunks);
+    const int *tok = a.tokens ? a.tokens + n * a.L : nullptr;
+    int pre[ADJ_PRE], step_len = 0;
+    if (tok && a.tokens_len) {
+        step_len = a.tokens_len[n];
+#pragma unroll
+        for (int i = 0; i < ADJ_PRE; ++i) pre[i] = tid + i * threads < a.L ? __ldg(tok + tid + i * threads) : -1;
+    }
+    const float rho = a.rho_n ? a.rho_n[n] : a.rho;
+    const float presence = a.presence_n ? a.presence_n[n] : a.presence;
+    const float frequency = a.frequency_n ? a.frequency_n[n] : a.frequency;
+    const int Tn = a.lx ? max(0, min(a.lx[n], a.T)) : a.T;
+    const int Un = a.ly ? max(0, min(a.ly[n], a.U1 - 1)) + 1 : a.U1;
+    const int V = a.V, plane = a.U1 * V, valid = Un * V;      // rows u < Un are the plane's first elements
+    const int limit = a.cu ? valid : plane;                   // elements of a frame in memory
+    const int ts = a.classes, run = chunk / ts;
+    const int ta = run * (a.tspan * ts) + (chunk - run * ts), tb = min((run + 1) * (a.tspan * ts), a.T), te = max(ta, min(tb, Tn));
+    const int64_t base = a.cu ? a.cu[n] * V : n * a.T * static_cast<int64_t>(plane), pitch = limit;
+    const int shift = static_cast<int>((base + ta * pitch) & (VE - 1));
+    const int p_tile = static_cast<int>(tile) * threads * VE - shift, p0 = p_tile + tid * VE;
+    const int lo = max(p0, 0), hi = min(p0 + VE, limit);
+    const bool whole = hi - lo == VE;
+    const bool work = ta < te && p_tile < valid;
+    const T *x = static_cast<const T *>(a.x) + base, *from = GRAD ? static_cast<const T *>(a.dy) + base : x;
+    const int64_t total = a.cu ? a.packed_rows * V - base : 0;   // a packed tensor may end inside a frame
+    // frames from which on the vector is not all inside the tensor
+    const int t_vec = !whole ? ta : a.cu ? static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(te), (total - hi) >= 0 ? (total - hi) / max(pitch, static_cast<int64_t>(1)) + 1 : 0))) : te;
+    Raw<T, VE> in[ADJ_UNROLL];
+    auto fetch = [&](int t) {
+#pragma unroll
+        for (int k = 0; k < ADJ_UNROLL; ++k)
+            if (t + k * ts < t_vec) in[k] = load_once<T, VE>(from + (t + k * ts) * pitch + p0);
+    };
+    fetch(ta);
+    float add[VE];
+    unsigned ok = 0, hit = 0;   // allowed; row exists and token stands in the history
+#pragma unroll
+    for (int e = 0; e < VE; ++e) add[e] = 0.0f;
+    if (work && lo < min(hi, valid)) {
+        int u = lo / V, v = lo - u * V;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+            if (p0 + e < lo || p0 + e >= valid) continue;
+            bool allow = true;
+            if (a.allowed) allow = a.allowed[n * a.mask_sn + u * a.mask_su + (v >> 5)] >> (v & 31) & 1u;
+            if (!GRAD && a.bias) {
+                const int64_t at = n * a.bias_sn + u * a.bias_su + v;
+                add[e] = a.bias_f32 ? static_cast<const float *>(a.bias)[at] : to_float(static_cast<const T *>(a.bias)[at]);
+            }
+            if (allow) ok |= 1u << e;
+            if (++v == V) {
+                v = 0;
+                ++u;
+            }
+        }
+    }
+    const bool history = work && tok;
+    if (history) {  // the same for the whole block
+        for (int i = tid; i < threads * VE / 4; i += threads) reinterpret_cast<int4 *>(count)[i] = make_int4(0, 0, 0, 0);
+        __syncthreads();
+        auto note = [&](int row, int v) {   // `row`: place of the row's first element in the tile, may be negative
+            if (v < 0 || v >= V) return;    // no token: ignored
+            const int to = row + v;
+            if (to >= 0 && to < threads * VE) atomicAdd(count + to, 1);
+        };
+        if (a.tokens_len) {
+            const int len = max(0, min(step_len, static_cast<int>(a.L)));
+#pragma unroll
+            for (int i = 0; i < ADJ_PRE; ++i)
+                if (tid + i * threads < len) note(-p_tile, pre[i]);
+            for (int j = tid + ADJ_PRE * threads; j < len; j += threads) note(-p_tile, tok[j]);
+        } else {
+            const int last = min((p_tile + threads * VE - 1) / V, Un - 1);
+            for (int r = max(p_tile, 0) / V; r <= last; ++r)
+                for (int j = tid; j < r; j += threads) note(r * V - p_tile, tok[j]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < VE; e += 4) {
+            const int4 c4 = *reinterpret_cast<const int4 *>(&count[tid * VE + e]);
+            const int times[4] = {c4.x, c4.y, c4.z, c4.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (times[i] > 0) {
+                    hit |= 1u << (e + i);
+                    add[e + i] -= presence + frequency * static_cast<float>(times[i]);
+                }
+        }
+    }
+    const int pad_from = valid - p0;   // elements from here on are padding rows: zeros
+    const bool scaled = hit && rho != 1.0f;
+    const float inv_rho = scaled ? 1.0f / rho : 1.0f;
+    float db[GRAD ? VE : 1];
+#pragma unroll
+    for (int e = 0; e < (GRAD ? VE : 1); ++e) db[e] = 0.0f;
+    const float ninf = -__int_as_float(0x7f800000);
+    auto one = [&](int e, float z, float xv) {   // element e: the logit, or its gradient and the logit
+        if (e >= pad_from) return 0.0f;
+        const bool allow = ok >> e & 1u;
+        if (GRAD) {
+            if (!allow) z = 0.0f;
+            db[GRAD ? e : 0] += z;
+            return (hit & ok) >> e & 1u ? z * (xv > 0.0f ? inv_rho : rho) : z;
+        }
+        if (scaled && (hit >> e & 1u)) z *= z > 0.0f ? inv_rho : rho;
+        return allow ? z + add[e] : ninf;
+    };
+    for (int t = ta; t < te; t += ADJ_UNROLL * ts) {
+        if (t > ta) fetch(t);
+        if (GRAD && scaled && out) {   // a thread reads back what it copied itself: no barrier, and no registers
+#pragma unroll
+            for (int k = 0; k < ADJ_UNROLL; ++k)
+                if (t + k * ts < t_vec) cp_async16(xs + k * ADJ_THREADS + tid, x + (t + k * ts) * pitch + p0);
+            cp_async_commit();
+            cp_async_wait<0>();
+        }
+#pragma unroll
+        for (int k = 0; k < ADJ_UNROLL; ++k) {
+            const int tk = t + k * ts;
+            if (tk >= te || lo >= hi) continue;
+            const int64_t o = tk * pitch + p0;
+            if (tk < t_vec) {
+                float z[VE], xv[VE];
+                unpack<T, VE>(in[k], z);
+#pragma unroll
+                for (int e = 0; e < VE; ++e) xv[e] = 0.0f;
+                if (GRAD && scaled && out) {
+                    Raw<T, VE> rx;
+                    memcpy(&rx, &xs[GRAD ? k * ADJ_THREADS + tid : 0], sizeof(rx));
+                    unpack<T, VE>(rx, xv);
+                }
+#pragma unroll
+                for (int e = 0; e < VE; ++e) z[e] = one(e, z[e], xv[e]);
+                if (!GRAD || out) store_raw<T, VE>(out + base + o, pack<T, VE>(z));
+            } else {
+#pragma unroll
+                for (int e = 0; e < VE; ++e) {
+                    if (p0 + e < lo || p0 + e >= hi || (a.cu && o + e >= total)) continue;
+                    const float r = one(e, to_float(from[o + e]), GRAD && scaled && out ? to_float(x[o + e]) : 0.0f);
+                    if (!GRAD || out) out[base + o + e] = from_float<T>(r);
+                }
+            }
+        }
+    }
+    if (!a.cu && out && lo < hi)   // frames behind the last one are zeros
+        for (int t = ta; t < tb; t += ts) {
+            if (t < te) continue;
+            if (whole) {
+                store_raw<T, VE>(out + base + t * pitch + p0, zero);
+            } else {
+                for (int p = lo; p < hi; ++p) out[base + t * pitch + p] = from_float<T>(0.0f);
+            }
+        }
+    if (GRAD && a.part) {
+        float *p = a.part + (n * a.chunks + chunk) * plane + p0;
+#pragma unroll
+        for (int e = 0; e < VE; ++e)
+            if (p0 + e >= 0 && p0 + e < plane) p[e] = db[GRAD ? e : 0];
     }
 }
 

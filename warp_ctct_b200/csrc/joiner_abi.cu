@@ -212,16 +212,19 @@ void jn_launch(const JnGeom &g, bool vec, const JnArgs &a, unsigned grid, cudaSt
 }
 // ---- adjustment of logits ----
 // Frames of a block: enough blocks for a few waves, and as many frames as that leaves, since the set-up of a
-// block (histories, bias, mask) is paid once for all its frames.
+// block (histories, bias, mask) is paid once for all its frames.  Where planes of U1 V elements (packed: rows of V) are no
+// whole number of vectors, frames come in classes that begin at the same place inside a vector.
 struct AdjGeom {
-    int64_t tspan, chunks;
+    int64_t tspan, chunks, classes;
 };
-AdjGeom adj_geom(int64_t N, int64_t T, int64_t U1, int64_t V) {
+AdjGeom adj_geom(int64_t N, int64_t T, int64_t U1, int64_t V, int dtype, bool packed) {
     AdjGeom g;
+    const int64_t E = 16 / static_cast<int64_t>(esize(dtype));
+    g.classes = (packed ? V : U1 * V) % E == 0 ? 1 : T < E ? (T < 1 ? 1 : T) : E;
     const int64_t tiles = ceil_div(U1 * V, 1024);
     g.tspan = 64;
-    while (g.tspan > ADJ_UNROLL && N * tiles * ceil_div(T, g.tspan) < 16 * kSms) g.tspan /= 2;
-    g.chunks = T > 0 ? ceil_div(T, g.tspan) : 1;
+    while (g.tspan > ADJ_UNROLL && N * tiles * g.classes * ceil_div(T, g.tspan * g.classes) < 16 * kSms) g.tspan /= 2;
+    g.chunks = T > 0 ? ceil_div(T, g.tspan * g.classes) * g.classes : 1;
     return g;
 }
 // Partial sums of the bias gradient: `outer` results of `P` partials of `C` columns.  Up to ADJ_FEW partials a thread
@@ -233,8 +236,8 @@ struct AdjReduce {
     int64_t outer, P, C, segments;
     size_t parts, total;   // bytes: partial sums, and with the runs behind them
 };
-AdjReduce adj_reduce(int64_t N, int64_t T, int64_t U1, int64_t V, int bias_kind) {
-    const int64_t chunks = adj_geom(N, T, U1, V).chunks;
+AdjReduce adj_reduce(int64_t N, int64_t T, int64_t U1, int64_t V, int dtype, bool packed, int bias_kind) {
+    const int64_t chunks = adj_geom(N, T, U1, V, dtype, packed).chunks;
     AdjReduce r;
     r.outer = bias_kind == 1 ? 1 : N;
     r.P = bias_kind == 1 ? N * chunks * U1 : bias_kind == 2 ? chunks * U1 : chunks;
@@ -250,23 +253,27 @@ bool adj_dims_ok(int64_t N, int64_t T, int64_t U1, int64_t V) {
     return N >= 0 && N <= kMaxGrid && T >= 0 && U1 >= 1 && V >= 1 && U1 < (int64_t(1) << 31) && V < (int64_t(1) << 31) &&
            T < (int64_t(1) << 31) && U1 * V < (int64_t(1) << 31) - 4096;
 }
+// `vec`: rows are whole vectors; `flat`: they are not, but the tensors begin with one and their rows follow one another
 template <typename T, bool GRAD>
-int adj_launch(AdjArgs &a, bool vec, int64_t N, bool tail, cudaStream_t st) {
+int adj_launch(AdjArgs &a, bool vec, bool flat, int64_t N, bool tail, cudaStream_t st) {
     constexpr int VE = 16 / static_cast<int>(sizeof(T));
     const int64_t plane = static_cast<int64_t>(a.U1) * a.V;
     // one row per n: a decoder's step
     const bool step = a.T == 1 && a.U1 == 1 && !a.cu && !a.lx && !a.ly && (!a.tokens || a.tokens_len);
-    const int64_t per = step ? (vec ? 2 * VE : 8) : vec ? VE : 4;   // elements of a thread
-    const int64_t need = ceil_div(plane, per);
+    // which has one frame to pay the set-up of an element with: odd rows go element by element (256 x 32001 bf16: 27 us, not 44)
+    if (step) flat = false;
+    const int64_t per = vec ? (step ? 2 * VE : VE) : flat ? VE : step ? 8 : 4;   // elements of a thread
+    const int64_t span = vec || !flat ? plane : plane + VE - 1;                  // a run may begin inside a vector
+    const int64_t need = ceil_div(span, per);
     const int threads = need < ADJ_THREADS ? static_cast<int>(ceil_div(need, 32) * 32) : ADJ_THREADS;
-    a.tiles = static_cast<int>(ceil_div(plane, threads * per));
+    a.tiles = static_cast<int>(ceil_div(span, threads * per));
     const int64_t blocks = N * a.tiles * a.chunks;
     if (blocks > kMaxGrid - 64) return CTCT_ERR_UNSUPPORTED;
     a.main_blocks = static_cast<unsigned>(blocks);
-    auto kernel = step ? (vec ? k_adjust<T, VE, 2, GRAD, true> : k_adjust<T, 1, 8, GRAD, true>)
-                       : (vec ? k_adjust<T, VE, 1, GRAD, false> : k_adjust<T, 1, 4, GRAD, false>);
-    launch_pdl(kernel, dim3(static_cast<unsigned>(blocks + (tail ? 16 : 0))),
-               dim3(threads), 0, st, a);
+    auto kernel = vec    ? (step ? k_adjust<T, VE, 2, GRAD, true> : k_adjust<T, VE, 1, GRAD, false>)
+                  : flat ? k_adjust_flat<T, GRAD>
+                         : (step ? k_adjust<T, 1, 8, GRAD, true> : k_adjust<T, 1, 4, GRAD, false>);
+    launch_pdl(kernel, dim3(static_cast<unsigned>(blocks + (tail ? 16 : 0))), dim3(threads), 0, st, a);
     return check_launch("adjust");
 }
 
@@ -463,9 +470,9 @@ int ctct_b200_joint_norm_backward(const void *dy, const void *f, int64_t f_sn, i
     });
 }
 
-size_t ctct_b200_adjust_workspace_bytes(int64_t N, int64_t T, int64_t U1, int64_t V, int bias_kind) {
-    if (!adj_dims_ok(N, T, U1, V) || bias_kind < 1 || bias_kind > 3) return 0;
-    return adj_reduce(N, T, U1, V, bias_kind).total;
+size_t ctct_b200_adjust_workspace_bytes(int64_t N, int64_t T, int64_t U1, int64_t V, int dtype, int packed, int bias_kind) {
+    if (!adj_dims_ok(N, T, U1, V) || !dtype_ok(dtype) || bias_kind < 1 || bias_kind > 3) return 0;
+    return adj_reduce(N, T, U1, V, dtype, packed != 0, bias_kind).total;
 }
 
 namespace {
@@ -518,9 +525,10 @@ int adj_fill(const AdjCall &c, int dtype, AdjArgs *a) {
     a->T = static_cast<int>(c.T);
     a->U1 = static_cast<int>(c.U1);
     a->V = static_cast<int>(c.V);
-    const AdjGeom g = adj_geom(c.N, c.T, c.U1, c.V);
+    const AdjGeom g = adj_geom(c.N, c.T, c.U1, c.V, dtype, c.packed_rows >= 0);
     a->tspan = static_cast<int>(g.tspan);
     a->chunks = static_cast<int>(g.chunks);
+    a->classes = static_cast<int>(g.classes);
     return CTCT_OK;
 }
 
@@ -547,9 +555,11 @@ int ctct_b200_adjust_forward(const void *logits, int64_t row_stride, int dtype, 
     a.y = out;
     const size_t es = esize(dtype);
     const int64_t E = 16 / static_cast<int64_t>(es);
-    const bool vec = V % E == 0 && row_stride % E == 0 && aligned(logits, 16) && aligned(out, 16) && aligned(bias, 16);
+    const bool base_ok = aligned(logits, 16) && aligned(out, 16);
+    const bool vec = V % E == 0 && row_stride % E == 0 && base_ok && aligned(bias, 16);
+    const bool flat = base_ok && (row_stride == 0 || row_stride == V);
     return with_type(dtype, [&](auto t) {
-        return adj_launch<decltype(t), false>(a, vec, N, packed_rows >= 0, static_cast<cudaStream_t>(stream));
+        return adj_launch<decltype(t), false>(a, vec, flat, N, packed_rows >= 0, static_cast<cudaStream_t>(stream));
     });
 }
 
@@ -564,7 +574,7 @@ int ctct_b200_adjust_backward(const void *dy, const void *logits, int64_t row_st
     if (int rc = adj_fill(c, dtype, &a)) return rc;
     if ((dbias && bias_kind == 0) || row_stride < 0 || (row_stride > 0 && (T != 1 || U1 != 1 || packed_rows >= 0))) return CTCT_ERR_ARG;
     const int64_t rows = packed_rows >= 0 ? packed_rows : N * T * U1;
-    const AdjReduce red = adj_reduce(N, T, U1, V, bias_kind);
+    const AdjReduce red = adj_reduce(N, T, U1, V, dtype, packed_rows >= 0, bias_kind);
     // one partial sum, laid out like the result: the blocks write the result themselves
     const bool direct = dbias && red.P == 1 && a.bias_f32;
     if (rows > 0 && (!dy || (dx && a.tokens && (repetition_n || repetition != 1.0f) && !logits))) return CTCT_ERR_ARG;
@@ -576,13 +586,15 @@ int ctct_b200_adjust_backward(const void *dy, const void *logits, int64_t row_st
     a.part = dbias ? static_cast<float *>(direct ? dbias : workspace) : nullptr;
     const size_t es = esize(dtype);
     const int64_t E = 16 / static_cast<int64_t>(es);
-    const bool vec = V % E == 0 && row_stride % E == 0 && aligned(logits, 16) && aligned(dx, 16) && aligned(dy, 16) && aligned(a.part, 16);
+    const bool base_ok = aligned(logits, 16) && aligned(dx, 16) && aligned(dy, 16);
+    const bool vec = V % E == 0 && row_stride % E == 0 && base_ok && aligned(a.part, 16);
+    const bool flat = base_ok && (row_stride == 0 || row_stride == V);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     return with_type(dtype, [&](auto t) -> int {
         using T_ = decltype(t);
         const bool some = rows > 0 && N * T > 0;
         if (some)
-            if (int rc = adj_launch<T_, true>(a, vec, N, packed_rows >= 0 && dx, st)) return rc;
+            if (int rc = adj_launch<T_, true>(a, vec, flat, N, packed_rows >= 0 && dx, st)) return rc;
         if (!dbias || (direct && some) || red.outer == 0) return CTCT_OK;
         float *parts = static_cast<float *>(workspace), *runs = some ? parts + red.parts / 4 : nullptr;
         ReduceArgs r{parts, dbias, a.bias_f32, some ? red.P : 0, red.C};   // no row: zeros

@@ -14,7 +14,7 @@ from typing import Optional
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import _lib
+from . import _as_int, _lib
 
 T = torch.Tensor
 
@@ -246,7 +246,6 @@ _joint_backward_once = once_differentiable(_joint_backward)
 
 
 def _joint(f: T, g: T, lx: Optional[T], ly: Optional[T], weight: Optional[T], bias: Optional[T], eps: float, rows: int) -> T:
-    from . import _as_int
     if not f.is_cuda:
         raise RuntimeError("f must be located in the CUDA")
     if not g.is_cuda:
