@@ -91,6 +91,13 @@ __device__ __forceinline__ Raw<T, VE> pack(const float *x) {
     return raw;
 }
 
+// 16 bytes into shared memory, or zeros without a look at `src`
+__device__ __forceinline__ void cp_async16_or_zero(void *dst, const void *src, bool there) {
+    const unsigned to = static_cast<unsigned>(__cvta_generic_to_shared(dst));
+    const int bytes = there ? 16 : 0;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src), "r"(bytes) : "memory");
+}
+
 // VE values of a parameter vector stored in float32 or in the activations' type T
 template <typename T, int VE>
 __device__ __forceinline__ void load_param(const void *p, int is_f32, int64_t at, float *v) {

@@ -3,6 +3,8 @@
 // workspace carving and launches; nothing here allocates or synchronises.
 #include "../../include/ctct_b200.h"
 
+#include <type_traits>
+
 #include "adjust.cuh"
 #include "elem.cuh"
 #include "jointnorm.cuh"
@@ -36,46 +38,51 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // Elements of a row per thread: 8 up to 256 per row (a warp each), else 16; float32 rows stay at 8 as long as
 // 512 threads cover the row, since 16 float32 of x and dy and their successors do not fit 128 registers.
 int ln_elems(int64_t H, int dtype) { return H <= 256 || (dtype == CTCT_F32 && H <= 8 * LN_WIDE_THREADS) ? 8 : 16; }
+// Threads per SM: forward 1024 (85 us at 16000 x 4096 f32, 110 with 512).  Backward as many as its registers leave (up to 148
+// a thread with 16 elements), so that all blocks run at a time; every block leaves a partial row of the weights'
+// gradients (16000 x 1024 bf16: 29 us, 40 with twice the blocks).
+constexpr int LN_FORWARD_THREADS = 1024;
+int ln_backward_threads(int P, bool wide, int dtype) { return wide ? 512 : P == 16 ? 384 : dtype == CTCT_F32 ? 512 : 640; }
 struct LnGeom {
     int P;
     bool wide, is_long;
     int threads;
     int64_t grid;
 };
-#ifndef LN_FT
-#define LN_FT 1024
-#endif
-#ifndef LN_BT
-#define LN_BT 512
-#endif
-LnGeom ln_geom(int64_t rows, int64_t H, int dtype, int per_sm) {
+LnGeom ln_geom(int64_t rows, int64_t H, int dtype, bool backward) {
+    const int64_t E = 16 / static_cast<int64_t>(esize(dtype));
+    const int64_t span = H % E == 0 ? H : H + E - 1;   // a row may begin inside a vector
     LnGeom g;
-    g.P = ln_elems(H, dtype);
-    g.is_long = H > static_cast<int64_t>(g.P) * LN_WIDE_THREADS;
-    g.wide = H > 32 * g.P;
-    g.threads = g.is_long ? LN_WIDE_THREADS : g.wide ? static_cast<int>(ceil_div(H, 32 * g.P)) * 32 : 32 * LN_WARPS;
-    // resident blocks: 512 threads' worth per SM
+    g.P = ln_elems(span, dtype);
+    g.is_long = span > static_cast<int64_t>(g.P) * LN_WIDE_THREADS;
+    g.wide = span > 32 * g.P;
+    g.threads = g.is_long ? LN_WIDE_THREADS : g.wide ? static_cast<int>(ceil_div(span, 32 * g.P)) * 32 : 32 * LN_WARPS;
     const int64_t blocks = g.wide ? rows : ceil_div(rows, LN_WARPS);
+    const int per_sm = backward ? ln_backward_threads(g.P, g.wide, dtype) : LN_FORWARD_THREADS;
     const int64_t most = static_cast<int64_t>(kSms) * (per_sm / g.threads > 0 ? per_sm / g.threads : 1);
     g.grid = blocks < most ? blocks : most;
+    // a block's rows are the grid apart: a multiple of a vector's elements where they begin inside vectors
+    if (H % E != 0 && !g.is_long) g.grid = g.grid < most ? ceil_div(g.grid, E) * E : g.grid / E * E;
     return g;
 }
 
-template <typename T, int VE, int P>
-void ln_launch(const LnGeom &g, const LnArgs &a, cudaStream_t st) {
-    const dim3 grid(static_cast<unsigned>(g.grid)), block(g.threads);
-    if (g.wide)
-        launch_pdl(k_ln_forward<T, VE, P, true>, grid, block, 0, st, a);
-    else
-        launch_pdl(k_ln_forward<T, VE, P, false>, grid, block, 0, st, a);
-}
-template <typename T, int VE, int P>
-void ln_launch(const LnGeom &g, const LnGradArgs &a, cudaStream_t st) {
-    const dim3 grid(static_cast<unsigned>(g.grid)), block(g.threads);
-    if (g.wide)
-        launch_pdl(k_ln_backward<T, VE, P, true>, grid, block, 0, st, a);
-    else
-        launch_pdl(k_ln_backward<T, VE, P, false>, grid, block, 0, st, a);
+// `vec`: rows are whole vectors; `odd`: they are not, but follow one another from an aligned first one
+template <typename T, int P, typename Args>
+void ln_launch(const LnGeom &g, bool vec, bool odd, const Args &a, cudaStream_t st) {
+    constexpr int E = 16 / static_cast<int>(sizeof(T));
+    void (*kernel)(Args);
+    if constexpr (std::is_same<Args, LnArgs>::value) {
+        if (g.wide)
+            kernel = vec ? k_ln_forward<T, E, P, true, false> : odd ? k_ln_forward<T, E, P, true, true> : k_ln_forward<T, 1, P, true, false>;
+        else
+            kernel = vec ? k_ln_forward<T, E, P, false, false> : odd ? k_ln_forward<T, E, P, false, true> : k_ln_forward<T, 1, P, false, false>;
+    } else {
+        if (g.wide)
+            kernel = vec ? k_ln_backward<T, E, P, true, false> : odd ? k_ln_backward<T, E, P, true, true> : k_ln_backward<T, 1, P, true, false>;
+        else
+            kernel = vec ? k_ln_backward<T, E, P, false, false> : odd ? k_ln_backward<T, E, P, false, true> : k_ln_backward<T, 1, P, false, false>;
+    }
+    launch_pdl(kernel, dim3(static_cast<unsigned>(g.grid)), dim3(g.threads), 0, st, a);
 }
 template <typename T, int VE>
 void ln_launch_long(const LnGeom &g, const LnArgs &a, cudaStream_t st) {
@@ -86,14 +93,14 @@ void ln_launch_long(const LnGeom &g, const LnGradArgs &a, cudaStream_t st) {
     launch_pdl(k_ln_backward_long<T, VE>, dim3(static_cast<unsigned>(g.grid)), dim3(g.threads), 0, st, a);
 }
 template <typename T, typename Args>
-void ln_dispatch(const LnGeom &g, bool vec, const Args &a, cudaStream_t st) {
+void ln_dispatch(const LnGeom &g, bool vec, bool odd, const Args &a, cudaStream_t st) {
     constexpr int E = 16 / static_cast<int>(sizeof(T));
     if (g.is_long)
         vec ? ln_launch_long<T, E>(g, a, st) : ln_launch_long<T, 1>(g, a, st);
     else if (g.P == 8)
-        vec ? ln_launch<T, E, 8>(g, a, st) : ln_launch<T, 1, 8>(g, a, st);
+        ln_launch<T, 8>(g, vec, odd, a, st);
     else
-        vec ? ln_launch<T, E, 16>(g, a, st) : ln_launch<T, 1, 16>(g, a, st);
+        ln_launch<T, 16>(g, vec, odd, a, st);
 }
 
 // ---- the additive joiner's layer norm ----
@@ -283,7 +290,7 @@ extern "C" {
 
 size_t ctct_b200_layer_norm_workspace_bytes(int64_t rows, int64_t H, int dtype) {
     if (rows < 0 || H < 1 || H >= (int64_t(1) << 31) || !dtype_ok(dtype)) return 0;
-    return align256(2 * static_cast<size_t>(ln_geom(rows, H, dtype, LN_BT).grid) * H * 4);
+    return align256(2 * static_cast<size_t>(ln_geom(rows, H, dtype, true).grid) * H * 4);
 }
 
 int ctct_b200_layer_norm_forward(const void *x, int64_t x_stride, int dtype, int64_t rows, int64_t H, const void *weight,
@@ -292,13 +299,14 @@ int ctct_b200_layer_norm_forward(const void *x, int64_t x_stride, int dtype, int
     if (rows == 0) return CTCT_OK;
     const size_t es = esize(dtype);
     const int64_t E = 16 / static_cast<int64_t>(es);
-    const bool vec = H % E == 0 && x_stride % E == 0 && aligned(x, 16) && aligned(y, 16) && aligned(weight, 16) &&
-                     aligned(bias, 16);
+    const bool base_ok = aligned(x, 16) && aligned(y, 16);
+    const bool vec = H % E == 0 && x_stride % E == 0 && base_ok && aligned(weight, 16) && aligned(bias, 16);
+    const bool odd = H % E != 0 && x_stride == H && base_ok;
     LnArgs a{x, x_stride, weight, bias, param_f32 || dtype == CTCT_F32, eps, y, reinterpret_cast<float2 *>(stats), rows,
              static_cast<int>(H)};
-    const LnGeom g = ln_geom(rows, H, dtype, LN_FT);
+    const LnGeom g = ln_geom(rows, H, dtype, false);
     return with_type(dtype, [&](auto t) {
-        ln_dispatch<decltype(t)>(g, vec, a, static_cast<cudaStream_t>(stream));
+        ln_dispatch<decltype(t)>(g, vec, odd, a, static_cast<cudaStream_t>(stream));
         return check_launch("layer_norm");
     });
 }
@@ -309,20 +317,21 @@ int ctct_b200_layer_norm_backward(const void *dy, int64_t dy_stride, const void 
     if (rows < 0 || H < 1 || H >= (int64_t(1) << 31) || !dtype_ok(dtype) || (rows > 0 && (!dy || !x || !stats))) return CTCT_ERR_ARG;
     const bool params = dweight || dbias;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const LnGeom g = ln_geom(rows, H, dtype, LN_BT);
+    const LnGeom g = ln_geom(rows, H, dtype, true);
     if (params && rows > 0 && (!workspace || !aligned(workspace, 256) || workspace_bytes < 2 * static_cast<size_t>(g.grid) * H * 4))
         return CTCT_ERR_WORKSPACE;
     const size_t es = esize(dtype);
     const int64_t E = 16 / static_cast<int64_t>(es);
-    const bool vec = H % E == 0 && x_stride % E == 0 && dy_stride % E == 0 && aligned(x, 16) && aligned(dy, 16) && aligned(dx, 16) &&
-                     aligned(weight, 16);
+    const bool base_ok = aligned(x, 16) && aligned(dy, 16) && aligned(dx, 16);
+    const bool vec = H % E == 0 && x_stride % E == 0 && dy_stride % E == 0 && base_ok && aligned(weight, 16);
+    const bool odd = H % E != 0 && x_stride == H && dy_stride == H && base_ok;
     const int p_f32 = param_f32 || dtype == CTCT_F32;
     LnGradArgs a{dy, dy_stride, x, x_stride, weight, p_f32, reinterpret_cast<const float2 *>(stats), dx,
                  params ? static_cast<float *>(workspace) : nullptr, rows, static_cast<int>(H)};
     return with_type(dtype, [&](auto t) -> int {
         using T = decltype(t);
         if (rows > 0) {
-            ln_dispatch<T>(g, vec, a, st);
+            ln_dispatch<T>(g, vec, odd, a, st);
             if (int rc = check_launch("layer_norm_grad")) return rc;
         }
         if (!params) return CTCT_OK;

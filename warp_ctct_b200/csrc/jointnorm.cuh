@@ -538,27 +538,31 @@ __global__ void __maxnreg__(REGS) k_joint_norm_grad(const JnGradArgs a) {
 #pragma unroll
                 for (int i = 0; i < Q; ++i) A[k][i] = z2;
             int64_t row = base + static_cast<int64_t>(t0) * pitch + u0;   // of the first of the TF frames
-            const T *dy[TF];
-#pragma unroll
-            for (int k = 0; k < TF; ++k) dy[k] = static_cast<const T *>(a.dy) + row * s.H + k * pitch_h;
+            const T *dy = static_cast<const T *>(a.dy) + row * s.H;
             const T *gr = g + u0 * a.g_su;
             const float *my_r = a.rstd + row + static_cast<int64_t>(kl) * pitch;
             float *my_c = cs + (tid >> 5) * 2 * TF + (lane >> 2);   // this lane's of {c1 of TF frames, c2 of TF frames}
             // FULL: all frames and rows are there; threads without columns read column 0 with a weight of zero
             auto walk = [&](auto full_tag) {
                 constexpr bool FULL = decltype(full_tag)::value;
-                constexpr bool RING = FULL && VE * sizeof(T) == 16 && REGS > JG_WIDE_REGS;   // 1024 threads leave no room for it
+                constexpr bool RING = VE * sizeof(T) == 16 && REGS > JG_WIDE_REGS;   // 1024 threads leave no room for it
                 Raw<T, VE> rd[RING ? 1 : TF][NV], rg[NV];
                 int p_slot = 0, c_slot = 0;
-                auto issue = [&](bool some) {
+                auto issue = [&](bool some, int kn) {
                     if (some) {
                         uint4 *to = ring + p_slot * (TF * NV) * team;
 #pragma unroll
                         for (int k = 0; k < TF; ++k) {
 #pragma unroll
-                            for (int i = 0; i < NV; ++i) cp_async16(to + (k * NV + i) * team, dy[k] + at[i]);
-                            dy[k] += s.H;
+                            for (int i = 0; i < NV; ++i) {
+                                if (FULL)
+                                    cp_async16(to + (k * NV + i) * team, dy + k * pitch_h + at[i]);
+                                else   // rows that are not there are filled with zeros, and not read
+                                    cp_async16_or_zero(to + (k * NV + i) * team,
+                                                       k < kn ? dy + k * pitch_h + at[i] : static_cast<const T *>(a.dy), k < kn);
+                            }
                         }
+                        dy += s.H;
                     }
                     cp_async_commit();
                     p_slot = p_slot + 1 == JG_STAGES ? 0 : p_slot + 1;
@@ -573,13 +577,13 @@ __global__ void __maxnreg__(REGS) k_joint_norm_grad(const JnGradArgs a) {
 #pragma unroll
                     for (int i = 0; i < NV; ++i) {
                         if (FULL) {
-                            rd[k][i] = load_once<T, VE>(dy[k] + at[i]);
+                            rd[k][i] = load_once<T, VE>(dy + k * pitch_h + at[i]);
                         } else {
                             rd[k][i] = Raw<T, VE>{};
-                            if (in[i] && k < kn) rd[k][i] = load_once<T, VE>(dy[k] + at[i]);
+                            if (in[i] && k < kn) rd[k][i] = load_once<T, VE>(dy + k * pitch_h + at[i]);
                         }
                     }
-                    dy[k] += s.H;
+                    if (k == TF - 1) dy += s.H;
                 };
                 auto fetch_g = [&]() {
 #pragma unroll
@@ -589,7 +593,7 @@ __global__ void __maxnreg__(REGS) k_joint_norm_grad(const JnGradArgs a) {
                 int kn = inside(row);
                 if constexpr (RING) {
 #pragma unroll
-                    for (int i = 0; i < JG_STAGES - 1; ++i) issue(u0 + i < ue);
+                    for (int i = 0; i < JG_STAGES - 1; ++i) issue(u0 + i < ue, inside(row + i));
                 } else {
 #pragma unroll
                     for (int k = 0; k < TF; ++k) fetch_row(k, kn);
@@ -613,9 +617,9 @@ __global__ void __maxnreg__(REGS) k_joint_norm_grad(const JnGradArgs a) {
                     float v[2 * TF];
 #pragma unroll
                     for (int i = 0; i < Q; ++i) B[i] = z2;
-                    const uint4 *slot = ring + c_slot * (TF * NV) * team;
+                    [[maybe_unused]] const uint4 *slot = ring + c_slot * (TF * NV) * team;
                     if constexpr (RING) {
-                        issue(u + JG_STAGES - 1 < ue);
+                        issue(u + JG_STAGES - 1 < ue, FULL ? TF : inside(row - 1 + JG_STAGES - 1));
                         cp_async_wait<JG_STAGES - 1>();
                         c_slot = c_slot + 1 == JG_STAGES ? 0 : c_slot + 1;
                     }

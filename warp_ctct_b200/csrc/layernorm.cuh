@@ -42,39 +42,101 @@ struct LnGradArgs {
 constexpr int LN_WARPS = 4;          // rows (warps) per block of the narrow kernels
 constexpr int LN_WIDE_THREADS = 512; // largest block that shares one row
 
-// WIDE: all threads of the block share a row (thread i holds chunks i, i + blockDim.x, ...), else every
-// warp has its own.  P elements per thread in chunks of VE.
-template <typename T, int VE, int P, bool WIDE>
+// A thread's P columns of a row: chunks of VE neighbours, chunk i at (i * team + tid) * VE.  ODD: rows that are no whole number
+// of 16-byte vectors, one behind the other: chunks are the aligned vectors that a row lies in, so its first column stands
+// `shift` elements inside a vector.  A block's rows are a multiple of a vector's elements apart, so the shift
+// is the block's and a thread keeps its columns; only the row's two ends are accessed element by element.  (With
+// 2-byte accesses 16000 rows of 1023 bf16 took 37 us forward and 148 backward; rows of 1024 take 17 and 30.)
+template <typename T, int VE, int NV, bool ODD>
+struct LnCols {
+    int col[NV];
+    bool whole[NV], some[NV];
+    __device__ __forceinline__ LnCols(int team, int tid, int H, int64_t first_row) {
+        const int shift = ODD ? static_cast<int>((first_row * H) & (VE - 1)) : 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            col[i] = (i * team + tid) * VE - shift;
+            whole[i] = ODD ? col[i] >= 0 && col[i] + VE <= H : col[i] < H;
+            some[i] = ODD ? col[i] + VE > 0 && col[i] < H : whole[i];
+        }
+    }
+    __device__ __forceinline__ bool has(int i, int e, int H) const {
+        return ODD ? whole[i] || (col[i] + e >= 0 && col[i] + e < H) : whole[i];
+    }
+    // a chunk as it lies in memory: with the neighbouring rows' elements where the row has none, but for the tensor's last vector,
+    // which may end behind the tensor and is read element by element
+    __device__ __forceinline__ Raw<T, VE> load(int i, const T *row, int H, const T *end) const {
+        if (whole[i] || (ODD && some[i] && row + col[i] + VE <= end)) return load_once<T, VE>(row + col[i]);
+        Raw<T, VE> raw{};
+        if (ODD && some[i]) {
+            T t[VE];
+            memcpy(t, &raw, sizeof(raw));
+#pragma unroll
+            for (int e = 0; e < VE; ++e)
+                if (has(i, e, H)) t[e] = row[col[i] + e];
+            memcpy(&raw, t, sizeof(raw));
+        }
+        return raw;
+    }
+    // its values, zeros where there is no column
+    __device__ __forceinline__ void values(int i, const Raw<T, VE> &raw, int H, float *x) const {
+        unpack<T, VE>(raw, x);
+        if (ODD && !whole[i]) {
+#pragma unroll
+            for (int e = 0; e < VE; ++e)
+                if (!has(i, e, H)) x[e] = 0.0f;
+        }
+    }
+    __device__ __forceinline__ void store(int i, T *row, int H, const float (&v)[VE]) const {
+        if (whole[i]) {
+            store_raw<T, VE>(row + col[i], pack<T, VE>(v));
+        } else if (ODD && some[i]) {
+#pragma unroll
+            for (int e = 0; e < VE; ++e)
+                if (has(i, e, H)) row[col[i] + e] = from_float<T>(v[e]);
+        }
+    }
+    // a parameter vector's values at the columns; `none` where there is no column or no vector
+    __device__ __forceinline__ void param(const void *p, int is_f32, int H, float none, float (&v)[NV * VE]) const {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int e = 0; e < VE; ++e) v[i * VE + e] = none;
+            if (!p) continue;
+            if (ODD) {
+#pragma unroll
+                for (int e = 0; e < VE; ++e)
+                    if (has(i, e, H)) load_param<T, 1>(p, is_f32, col[i] + e, v + i * VE + e);
+            } else if (whole[i]) {
+                load_param<T, VE>(p, is_f32, col[i], v + i * VE);
+            }
+        }
+    }
+};
+
+// WIDE: all threads of the block share a row, else every warp has its own: rows blockIdx.x + gridDim.x * k, k dealt to the
+// warps in turn.
+template <typename T, int VE, int P, bool WIDE, bool ODD>
 __global__ void __launch_bounds__(WIDE ? LN_WIDE_THREADS : 32 * LN_WARPS) k_ln_forward(const LnArgs a) {
     constexpr int NV = P / VE;
     __shared__ float sm[2 * 32];
     pdl_wait();
     const int team = WIDE ? blockDim.x : 32, tid = WIDE ? threadIdx.x : (threadIdx.x & 31);
     const int64_t step = WIDE ? gridDim.x : static_cast<int64_t>(gridDim.x) * LN_WARPS;
-    int64_t row = WIDE ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * LN_WARPS + (threadIdx.x >> 5);
+    int64_t row = blockIdx.x + (WIDE ? 0 : static_cast<int64_t>(threadIdx.x >> 5) * gridDim.x);
     const float inv_h = 1.0f / static_cast<float>(a.H);
+    const LnCols<T, VE, NV, ODD> c(team, tid, a.H, row);
+    const T *const x_end = static_cast<const T *>(a.x) + a.rows * a.H;   // of contiguous rows
     Raw<T, VE> raw[NV];
     auto fetch = [&](int64_t r) {
         const T *x = static_cast<const T *>(a.x) + r * a.x_stride;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int col = (i * team + tid) * VE;
-            if (col < a.H) raw[i] = load_once<T, VE>(x + col);
-        }
+        for (int i = 0; i < NV; ++i) raw[i] = c.load(i, x, a.H, x_end);
     };
     if (row < a.rows) fetch(row);
     float w[P], b[P];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int col = (i * team + tid) * VE;
-#pragma unroll
-        for (int e = 0; e < VE; ++e) {
-            w[i * VE + e] = 1.0f;
-            b[i * VE + e] = 0.0f;
-        }
-        if (col < a.H && a.w) load_param<T, VE>(a.w, a.p_f32, col, w + i * VE);
-        if (col < a.H && a.b) load_param<T, VE>(a.b, a.p_f32, col, b + i * VE);
-    }
+    c.param(a.w, a.p_f32, a.H, 1.0f, w);
+    c.param(a.b, a.p_f32, a.H, 0.0f, b);
     int slot = 0;
     auto total = [&](float v) {
         if (!WIDE) return warp_sum(v);
@@ -88,43 +150,43 @@ __global__ void __launch_bounds__(WIDE ? LN_WIDE_THREADS : 32 * LN_WARPS) k_ln_f
         float s = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            if ((i * team + tid) * VE < a.H) {
-                unpack<T, VE>(raw[i], x + i * VE);
+            c.values(i, raw[i], a.H, x + i * VE);
 #pragma unroll
-                for (int e = 0; e < VE; ++e) s += x[i * VE + e];
-            }
+            for (int e = 0; e < VE; ++e) s += x[i * VE + e];
         }
         if (row + step < a.rows) fetch(row + step);  // the next row is on its way during this one's sums
         const float mean = total(s) * inv_h;
         s = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            if ((i * team + tid) * VE < a.H) {
+            if (c.some[i]) {
 #pragma unroll
-                for (int e = 0; e < VE; ++e) {
-                    const float d = x[i * VE + e] - mean;
-                    x[i * VE + e] = d;
-                    s = fmaf(d, d, s);
+                for (int e = 0; e < VE; ++e) x[i * VE + e] -= mean;
+                if (ODD && !c.whole[i]) {
+#pragma unroll
+                    for (int e = 0; e < VE; ++e)
+                        if (!c.has(i, e, a.H)) x[i * VE + e] = 0.0f;
                 }
+#pragma unroll
+                for (int e = 0; e < VE; ++e) s = fmaf(x[i * VE + e], x[i * VE + e], s);
             }
         }
         const float rstd = rsqrtf(fmaf(total(s), inv_h, a.eps));
         T *y = static_cast<T *>(a.y) + row * a.H;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int col = (i * team + tid) * VE;
-            if (col < a.H) {
+            if (c.some[i]) {
                 float o[VE];
 #pragma unroll
                 for (int e = 0; e < VE; ++e) o[e] = fmaf(x[i * VE + e] * rstd, w[i * VE + e], b[i * VE + e]);
-                store_raw<T, VE>(y + col, pack<T, VE>(o));
+                c.store(i, y, a.H, o);
             }
         }
         if (a.stats && tid == 0) a.stats[row] = make_float2(mean, rstd);
     }
 }
 
-template <typename T, int VE, int P, bool WIDE>
+template <typename T, int VE, int P, bool WIDE, bool ODD>
 __global__ void __launch_bounds__(WIDE ? LN_WIDE_THREADS : 32 * LN_WARPS) k_ln_backward(const LnGradArgs a) {
     constexpr int NV = P / VE;
     __shared__ float sm[2 * 2 * 32];
@@ -132,8 +194,10 @@ __global__ void __launch_bounds__(WIDE ? LN_WIDE_THREADS : 32 * LN_WARPS) k_ln_b
     pdl_trigger();
     const int team = WIDE ? blockDim.x : 32, tid = WIDE ? threadIdx.x : (threadIdx.x & 31);
     const int64_t step = WIDE ? gridDim.x : static_cast<int64_t>(gridDim.x) * LN_WARPS;
-    int64_t row = WIDE ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * LN_WARPS + (threadIdx.x >> 5);
+    int64_t row = blockIdx.x + (WIDE ? 0 : static_cast<int64_t>(threadIdx.x >> 5) * gridDim.x);
     const float inv_h = 1.0f / static_cast<float>(a.H);
+    const LnCols<T, VE, NV, ODD> c(team, tid, a.H, row);
+    const T *const x_end = static_cast<const T *>(a.x) + a.rows * a.H, *const d_end = static_cast<const T *>(a.dy) + a.rows * a.H;
     Raw<T, VE> rx[NV], rd[NV];
     float2 st = make_float2(0.0f, 0.0f);
     auto fetch = [&](int64_t r) {
@@ -142,44 +206,32 @@ __global__ void __launch_bounds__(WIDE ? LN_WIDE_THREADS : 32 * LN_WARPS) k_ln_b
         st = a.stats[r];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int col = (i * team + tid) * VE;
-            if (col < a.H) {
-                rx[i] = load_once<T, VE>(x + col);
-                rd[i] = load_once<T, VE>(d + col);
-            }
+            rx[i] = c.load(i, x, a.H, x_end);
+            rd[i] = c.load(i, d, a.H, d_end);
         }
     };
     if (row < a.rows) fetch(row);
     float w[P], dw[P], db[P];
+    c.param(a.w, a.p_f32, a.H, 1.0f, w);
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
-        w[i] = 1.0f;
-        dw[i] = db[i] = 0.0f;
-    }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int col = (i * team + tid) * VE;
-        if (col < a.H && a.w) load_param<T, VE>(a.w, a.p_f32, col, w + i * VE);
-    }
+    for (int i = 0; i < P; ++i) dw[i] = db[i] = 0.0f;
     int slot = 0;
     for (; row < a.rows; row += step) {
         float xh[P], d[P];
         const float rstd = st.y, mean = st.x;
         float sums[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            if ((i * team + tid) * VE < a.H) {
-                unpack<T, VE>(rx[i], xh + i * VE);
-                unpack<T, VE>(rd[i], d + i * VE);
+        for (int i = 0; i < NV; ++i) {   // where there is no column dy is zero, and so is all that it enters
+            c.values(i, rx[i], a.H, xh + i * VE);
+            c.values(i, rd[i], a.H, d + i * VE);
 #pragma unroll
-                for (int e = i * VE; e < (i + 1) * VE; ++e) {
-                    xh[e] = (xh[e] - mean) * rstd;
-                    const float q = w[e] * d[e];
-                    sums[0] += q;
-                    sums[1] = fmaf(q, xh[e], sums[1]);
-                    dw[e] = fmaf(d[e], xh[e], dw[e]);
-                    db[e] += d[e];
-                }
+            for (int e = i * VE; e < (i + 1) * VE; ++e) {
+                xh[e] = (xh[e] - mean) * rstd;
+                const float q = w[e] * d[e];
+                sums[0] += q;
+                sums[1] = fmaf(q, xh[e], sums[1]);
+                dw[e] = fmaf(d[e], xh[e], dw[e]);
+                db[e] += d[e];
             }
         }
         if (row + step < a.rows) fetch(row + step);
@@ -195,15 +247,14 @@ __global__ void __launch_bounds__(WIDE ? LN_WIDE_THREADS : 32 * LN_WARPS) k_ln_b
         T *dx = static_cast<T *>(a.dx) + row * a.H;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int col = (i * team + tid) * VE;
-            if (col < a.H) {
+            if (c.some[i]) {
                 float o[VE];
 #pragma unroll
                 for (int e = 0; e < VE; ++e) {
                     const int k = i * VE + e;
                     o[e] = (fmaf(w[k], d[k], -c1) - xh[k] * c2) * rstd;
                 }
-                store_raw<T, VE>(dx + col, pack<T, VE>(o));
+                c.store(i, dx, a.H, o);
             }
         }
     }
@@ -213,14 +264,12 @@ __global__ void __launch_bounds__(WIDE ? LN_WIDE_THREADS : 32 * LN_WARPS) k_ln_b
     if (WIDE) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int col = (i * team + tid) * VE;
-            if (col < a.H) {
 #pragma unroll
-                for (int e = 0; e < VE; ++e) {
-                    pw[col + e] = dw[i * VE + e];
-                    pb[col + e] = db[i * VE + e];
+            for (int e = 0; e < VE; ++e)
+                if (c.has(i, e, a.H)) {
+                    pw[c.col[i] + e] = dw[i * VE + e];
+                    pb[c.col[i] + e] = db[i * VE + e];
                 }
-            }
         }
     } else {  // join the rows of the block's warps, one warp after the other
         __shared__ float acc[2][32 * P];
@@ -234,12 +283,15 @@ __global__ void __launch_bounds__(WIDE ? LN_WIDE_THREADS : 32 * LN_WARPS) k_ln_b
             }
             __syncthreads();
         }
-        for (int i = threadIdx.x; i < 32 * P; i += 32 * LN_WARPS) {
-            // value i belongs to lane i % 32, its element i / 32
-            const int e = i / 32, col = ((e / VE) * 32 + (i & 31)) * VE + e % VE;
-            if (col < a.H) {
-                pw[col] = acc[0][i];
-                pb[col] = acc[1][i];
+        if (threadIdx.x < 32) {   // the first warp has the columns that all of them have
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+#pragma unroll
+                for (int e = 0; e < VE; ++e)
+                    if (c.has(i, e, a.H)) {
+                        pw[c.col[i] + e] = acc[0][(i * VE + e) * 32 + tid];
+                        pb[c.col[i] + e] = acc[1][(i * VE + e) * 32 + tid];
+                    }
             }
         }
     }
