@@ -349,7 +349,9 @@ constexpr int JG_P = 8, JG_TF = 4;      // columns per thread, frames per block 
 constexpr int JG_MAX_THREADS = 256;
 constexpr int JG_REGS = 168, JG_WIDE_REGS = 64;   // registers per thread up to JG_MAX_THREADS, and of the wide kernels
 constexpr int JG_BATCH = 8;             // contexts whose g is on its way together behind the stream
-constexpr int JG_BLOCKS = 16;           // most blocks of TF frames that a thread block takes
+// Most blocks of TF frames that a thread block takes.  Few mean many partial sums, many mean fewer contexts a block, whose
+// shared memory they share: 8, 16, 32 took 217, 189, 187 us at 32x256x65x512 bf16, 626, 541, 505 at 16x512x129x1024 fp16.
+constexpr int JG_BLOCKS = 32;
 constexpr int JG_STAGES = 2;            // of a thread's ring of rows of dy
 // Shared memory of a block (floats): B [uspan][P / 4][team][4] and dw [P / 2][team][2], private to the threads; c1 and c2
 // [uspan][warps][2 * TF];
