@@ -205,6 +205,29 @@ def test_joint(W, dtype, packed, shape, bias_kind, mask_kind):
         _check_bias("dbias", got[1], dz, bias, {1: (0, 1, 2), 2: (1, 2), 3: (1,)}[bias_kind], int(valid.sum()))
 
 
+@pytest.mark.parametrize("dtype,packed,V,bias_kind", [(torch.float32, False, 512, 1), (torch.float16, True, 509, 3), (torch.bfloat16, False, 510, 2),
+                                                      (torch.bfloat16, True, 264, 1), (torch.float32, True, 203, 1)])
+def test_joint_large(W, dtype, packed, V, bias_kind):
+    """Blocks that walk over many frames, and many partial sums of the bias gradient."""
+    test_joint(W, dtype, packed, (12, 300, 33, V), bias_kind, 3)
+
+
+def test_nothing_to_adjust(W):
+    """No rows, no frames: gradients of the bias are zeros; 64-bit tokens beyond 32 bits are no tokens."""
+    for shape in ((0, 5, 3, 8), (2, 0, 3, 8)):
+        x = torch.zeros(shape, device=DEV, requires_grad=True)
+        for bias_shape in ((8,), (shape[0], 8), (shape[0], 3, 8)):
+            b = torch.ones(bias_shape, device=DEV, requires_grad=True)
+            y = W.adjust_joint_logits(x, torch.ones((shape[0], 2), dtype=torch.int32, device=DEV), bias=b, repetition_penalty=1.5)
+            assert y.shape == shape
+            dx, db = torch.autograd.grad(y, [x, b], torch.ones_like(y))
+            assert dx.shape == shape and db.shape == b.shape and not db.any()
+    x = torch.randn((2, 9), device=DEV)
+    far = torch.tensor([[2 ** 32 + 3, -2 ** 40, 3], [2 ** 31 + 1, 2 ** 33, 4]], device=DEV)
+    near = torch.tensor([[3], [4]], device=DEV)
+    assert torch.equal(W.adjust_logits(x, far, None, None, None, 1.5, 0.5, 0.25), W.adjust_logits(x, near, None, None, None, 1.5, 0.5, 0.25))
+
+
 def test_joint_without_lengths_and_per_utterance_penalties(W):
     N, T, U1, V = 3, 14, 8, 50
     x, labels, _, _, bias, allowed, dy = _joint_case(W, 11, N, T, U1, V, torch.float32, 1, 2)

@@ -73,6 +73,15 @@ def test_layer_norm(W, dtype, rows, H):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,H", [(30000, 96), (20000, 520), (9001, 1031), (5003, 2047), (3000, 4100)])
+def test_layer_norm_many_rows(W, dtype, rows, H):
+    """More rows than the GPU has blocks: each takes several, and its share of the weights' gradients with it."""
+    g = _gen(rows)
+    _check_ln(W, _rand(g, (rows, H), dtype, 1.5, 0.5), _rand(g, (H,), torch.float32, 0.3, 1.0), _rand(g, (H,), torch.float32, 0.3), 1e-5,
+              _rand(g, (rows, H), dtype))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_layer_norm_without_parameters_and_with_one(W, dtype):
     g = _gen(3)
     x, dy = _rand(g, (37, 96), dtype), _rand(g, (37, 96), dtype)
@@ -194,6 +203,36 @@ def test_joint_layer_norm(W, dtype, packed, shape):
     N, T, U1, H = shape
     g, f, gg, w, b, lx, ly = _joint_args(sum(shape), N, T, U1, H, dtype, dtype if H % 2 else torch.float32, True)
     _check_joint(W, f, gg, lx, ly, w, b, 1e-5, _rand(g, (N, T, U1, H), dtype), packed)
+
+
+@pytest.mark.parametrize("dtype,packed,shape", [(torch.float32, True, (64, 128, 40, 64)), (torch.bfloat16, False, (64, 128, 40, 72)),
+                                                (torch.float16, True, (4, 200, 25, 1030)), (torch.bfloat16, False, (3, 260, 50, 2048)),
+                                                (torch.float32, False, (300, 30, 3, 40)), (torch.float16, True, (20, 150, 70, 96))])
+def test_joint_layer_norm_large_ragged_batches(W, dtype, packed, shape):
+    """More cells than blocks: runs of several, over ranges of contexts and over utterances, some of which have no frames."""
+    N, T, U1, H = shape
+    g, f, gg, w, b, lx, ly = _joint_args(sum(shape), N, T, U1, H, dtype, torch.float32, True)
+    lx[1:N - 1:3] = 0
+    lx[-1] = min(1, T)
+    _check_joint(W, f, gg, lx, ly, w, b, 1e-5, _rand(g, (N, T, U1, H), dtype), packed)
+
+
+def test_workspaces_may_hold_anything(W):
+    """Memory that the allocator hands out again full of NaN does not show, not even for utterances without frames."""
+    N, T, U1, H = 3, 9, 6, 64
+    g, f, gg, w, b, _, ly = _joint_args(8, N, T, U1, H, torch.float32, torch.float32, True)
+    lx = torch.tensor([9, 0, 4], dtype=torch.int32, device=DEV)
+    leaves = [t.requires_grad_(True) for t in (f, gg, w, b)]
+    first = None
+    for _ in range(3):
+        junk = [torch.full((k,), float("nan"), device=DEV) for k in (1 << 10, 1 << 12, 1 << 14, 1 << 16, 1 << 18, 1 << 20)]
+        del junk
+        y = W.joint_layer_norm(leaves[0], leaves[1], lx, ly, leaves[2], leaves[3])
+        got = [y.detach(), *torch.autograd.grad(y, leaves, torch.ones_like(y))]
+        assert all(bool(t.isfinite().all()) for t in got)
+        first = first or got
+        for p, q in zip(first, got):
+            assert torch.equal(p, q)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -182,6 +182,8 @@ def _int_on(name: str, t: T, device) -> T:
         return t if t.is_contiguous() else t.contiguous()
     if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
         raise RuntimeError(f"{name} must hold integers, not {t.dtype}")
+    if t.dtype == torch.int64:   # what 32 bits do not hold is out of every range, and stays so
+        t = t.clamp(-1, 2 ** 31 - 1)
     return t.to(torch.int32).contiguous()
 
 

@@ -160,7 +160,7 @@ bool jn_grad_geom(int64_t N, int64_t T, int64_t U1, int64_t H, int dtype, JnGeom
 }
 bool jn_dims_ok(int64_t N, int64_t T, int64_t U1, int64_t H) {
     return N >= 0 && N <= 65535 && T >= 0 && U1 >= 1 && H >= 1 && H < (int64_t(1) << 31) && T * U1 < (int64_t(1) << 31) &&
-           N * T * U1 < (int64_t(1) << 38);
+           N * T < (int64_t(1) << 31) && N * U1 < (int64_t(1) << 31) && N * T * U1 < (int64_t(1) << 38);
 }
 struct JnSaved {
     size_t cu, fm, gm, rstd, total;
@@ -500,11 +500,13 @@ struct AdjCall {
     const float *rho_n, *presence_n, *frequency_n;
 };
 // the common part of both directions; CTCT_OK, or why the call is refused
-int adj_fill(const AdjCall &c, int dtype, AdjArgs *a) {
+int adj_fill(const AdjCall &c, int dtype, bool forward, AdjArgs *a) {
     if (!adj_dims_ok(c.N, c.T, c.U1, c.V) || !dtype_ok(dtype)) return CTCT_ERR_ARG;
     if (c.packed_rows >= 0 && (!c.lx || !c.ly || !c.cu)) return CTCT_ERR_ARG;
     if (c.bias_kind < 0 || c.bias_kind > 3 || c.mask_kind < 0 || c.mask_kind > 3) return CTCT_ERR_ARG;
-    if ((c.mask_kind != 0) != (c.allowed != nullptr)) return CTCT_ERR_ARG;
+    const bool rows = c.packed_rows >= 0 ? c.packed_rows > 0 : c.N > 0 && c.T > 0;   // a tensor without elements may have no address
+    if (c.mask_kind == 0 ? c.allowed != nullptr : rows && !c.allowed) return CTCT_ERR_ARG;
+    if (forward && (c.bias_kind == 0 ? c.bias != nullptr : rows && !c.bias)) return CTCT_ERR_ARG;
     if (c.tokens_pitch < 0 || (c.tokens && !c.tokens_len && c.tokens_pitch < c.U1 - 1)) return CTCT_ERR_ARG;
     if (!c.rho_n && !(c.rho > 0.0f)) return CTCT_ERR_ARG;
     const int64_t words = ceil_div(c.V, 32);
@@ -551,8 +553,8 @@ int ctct_b200_adjust_forward(const void *logits, int64_t row_stride, int dtype, 
     AdjArgs a = {};
     const AdjCall c{tokens, tokens_lengths, tokens_pitch, lx, ly, N, T, U1, V, packed_rows, cu_rows, bias, bias_kind, bias_f32,
                     allowed, mask_kind, repetition, presence, frequency, repetition_n, presence_n, frequency_n};
-    if (int rc = adj_fill(c, dtype, &a)) return rc;
-    if ((bias_kind != 0) != (bias != nullptr) || row_stride < 0 || (row_stride > 0 && (T != 1 || U1 != 1 || packed_rows >= 0)))
+    if (int rc = adj_fill(c, dtype, true, &a)) return rc;
+    if (row_stride < 0 || (row_stride > 0 && (T != 1 || U1 != 1 || packed_rows >= 0)))
         return CTCT_ERR_ARG;
     const int64_t rows = packed_rows >= 0 ? packed_rows : N * T * U1;
     if (rows == 0) return CTCT_OK;
@@ -580,7 +582,7 @@ int ctct_b200_adjust_backward(const void *dy, const void *logits, int64_t row_st
     AdjArgs a = {};
     const AdjCall c{tokens, tokens_lengths, tokens_pitch, lx, ly, N, T, U1, V, packed_rows, cu_rows, nullptr, bias_kind, bias_f32,
                     allowed, mask_kind, repetition, 0.0f, 0.0f, repetition_n, nullptr, nullptr};
-    if (int rc = adj_fill(c, dtype, &a)) return rc;
+    if (int rc = adj_fill(c, dtype, false, &a)) return rc;
     if ((dbias && bias_kind == 0) || row_stride < 0 || (row_stride > 0 && (T != 1 || U1 != 1 || packed_rows >= 0))) return CTCT_ERR_ARG;
     const int64_t rows = packed_rows >= 0 ? packed_rows : N * T * U1;
     const AdjReduce red = adj_reduce(N, T, U1, V, dtype, packed_rows >= 0, bias_kind);
