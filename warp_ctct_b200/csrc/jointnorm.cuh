@@ -32,7 +32,6 @@
 
 namespace ctct {
 
-
 struct JnShape {
     const int *lx, *ly;      // frames and labels per utterance, or nullptr: all of them
     const int64_t *cu;       // packed: row offsets per utterance (N + 1); nullptr = padded

@@ -109,7 +109,7 @@ def _ln_backward(ctx, dy: T):
         if need_w:
             dw = torch.empty_like(weight)
         if need_b:
-            db = torch.empty((H,), dtype=bias_dtype, device=dev)
+            db = torch.empty((H,), dtype=bias_dtype, device=dev) if dw is None else torch.empty_like(dw)
         if need_w or need_b:
             nbytes = lib.ctct_b200_layer_norm_workspace_bytes(R, H, code)
             ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
@@ -209,10 +209,10 @@ def _joint_backward(ctx, dy: T):
     need_f, need_g, need_w, need_b = ctx.needs_input_grad[:4]
     prev = _lib.enter_device(dev)
     try:
-        df = f.new_empty((N, Tm, H)) if need_f else None
-        dg = f.new_empty((N, U1, H)) if need_g else None
+        df = None if not need_f else torch.empty_like(f) if f.is_contiguous() else f.new_empty((N, Tm, H))
+        dg = None if not need_g else torch.empty_like(g) if g.is_contiguous() else g.new_empty((N, U1, H))
         dw = torch.empty_like(weight) if need_w else None
-        db = torch.empty((H,), dtype=bias_dtype, device=dev) if need_b else None
+        db = None if not need_b else torch.empty((H,), dtype=bias_dtype, device=dev) if dw is None else torch.empty_like(dw)
         nbytes = lib.ctct_b200_joint_norm_workspace_bytes(N, Tm, U1, H, code)
         ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
         rc = lib.ctct_b200_joint_norm_backward(
