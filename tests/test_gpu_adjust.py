@@ -228,6 +228,42 @@ def test_nothing_to_adjust(W):
     assert torch.equal(W.adjust_logits(x, far, None, None, None, 1.5, 0.5, 0.25), W.adjust_logits(x, near, None, None, None, 1.5, 0.5, 0.25))
 
 
+@pytest.mark.parametrize("V", [24, 23])
+@pytest.mark.parametrize("bias_kind", [0, 1, 2, 3])
+def test_surplus_rows_without_any_frame(W, V, bias_kind):
+    """A packed tensor of surplus rows only: zeros, and so are their gradients, whatever the memory held."""
+    rows, N, U1 = 70, 2, 3
+    lengths = torch.zeros((N,), dtype=torch.int32, device=DEV)
+    labels = torch.ones((N, U1 - 1), dtype=torch.int32, device=DEV)
+    bias = torch.ones([(), (V,), (N, V), (N, U1, V)][bias_kind], device=DEV, requires_grad=True) if bias_kind else None
+    for max_frames in (0, 4):
+        x = torch.randn((rows, V), device=DEV, requires_grad=True)
+        y = W.adjust_joint_logits_packed(x, labels, lengths, lengths, max_frames=max_frames, bias=bias, repetition_penalty=1.5)
+        assert y.shape == x.shape and not y.any()
+        dy = torch.ones_like(y)
+        dirty = [torch.full((rows, V), float("nan"), device=DEV) for _ in range(4)]
+        del dirty
+        got = torch.autograd.grad(y, [x] + [bias] * (bias_kind > 0), dy)
+        assert not any(t.any() for t in got)
+
+
+@pytest.mark.parametrize("rows", [0, 5])
+def test_packed_without_utterances(W, rows):
+    none = torch.zeros((0,), dtype=torch.int32, device=DEV)
+    labels = torch.zeros((0, 2), dtype=torch.int32, device=DEV)
+    for dtype in (torch.float32, torch.bfloat16):
+        x = torch.randn((rows, 11), device=DEV).to(dtype).requires_grad_(True)
+        b = torch.ones((11,), device=DEV, requires_grad=True)
+        for max_frames in (None, 0, 6):
+            y = W.adjust_joint_logits_packed(x, labels, none, none, max_frames=max_frames, bias=b, repetition_penalty=1.5)
+            assert y.shape == x.shape and not y.any()
+            dx, db = torch.autograd.grad(y, [x, b], torch.ones_like(y))
+            assert dx.shape == x.shape and not dx.any() and not db.any()
+            only_b, = torch.autograd.grad(W.adjust_joint_logits_packed(x.detach(), labels, none, none, max_frames=max_frames, bias=b),
+                                          [b], torch.ones_like(y))
+            assert not only_b.any()
+
+
 def test_joint_without_lengths_and_per_utterance_penalties(W):
     N, T, U1, V = 3, 14, 8, 50
     x, labels, _, _, bias, allowed, dy = _joint_case(W, 11, N, T, U1, V, torch.float32, 1, 2)

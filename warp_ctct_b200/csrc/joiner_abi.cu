@@ -502,9 +502,9 @@ struct AdjCall {
 // the common part of both directions; CTCT_OK, or why the call is refused
 int adj_fill(const AdjCall &c, int dtype, bool forward, AdjArgs *a) {
     if (!adj_dims_ok(c.N, c.T, c.U1, c.V) || !dtype_ok(dtype)) return CTCT_ERR_ARG;
-    if (c.packed_rows >= 0 && (!c.lx || !c.ly || !c.cu)) return CTCT_ERR_ARG;
+    if (c.packed_rows >= 0 && (((!c.lx || !c.ly) && c.N > 0) || !c.cu)) return CTCT_ERR_ARG;
     if (c.bias_kind < 0 || c.bias_kind > 3 || c.mask_kind < 0 || c.mask_kind > 3) return CTCT_ERR_ARG;
-    const bool rows = c.packed_rows >= 0 ? c.packed_rows > 0 : c.N > 0 && c.T > 0;   // a tensor without elements may have no address
+    const bool rows = c.N > 0 && (c.packed_rows >= 0 ? c.packed_rows > 0 : c.T > 0);   // a tensor without elements may have no address
     if (c.mask_kind == 0 ? c.allowed != nullptr : rows && !c.allowed) return CTCT_ERR_ARG;
     if (forward && (c.bias_kind == 0 ? c.bias != nullptr : rows && !c.bias)) return CTCT_ERR_ARG;
     if (c.tokens_pitch < 0 || (c.tokens && !c.tokens_len && c.tokens_pitch < c.U1 - 1)) return CTCT_ERR_ARG;
@@ -589,7 +589,9 @@ int ctct_b200_adjust_backward(const void *dy, const void *logits, int64_t row_st
     // one partial sum, laid out like the result: the blocks write the result themselves
     const bool direct = dbias && red.P == 1 && a.bias_f32;
     if (rows > 0 && (!dy || (dx && a.tokens && (repetition_n || repetition != 1.0f) && !logits))) return CTCT_ERR_ARG;
-    if (rows > 0 && dbias && !direct && (!workspace || !aligned(workspace, 256) || workspace_bytes < red.total)) return CTCT_ERR_WORKSPACE;
+    // a packed tensor without frames has surplus rows only: no sums without utterances, but zeros in dx
+    const bool sums = rows > 0 && N > 0, some = sums || (rows > 0 && dx);
+    if (sums && dbias && !direct && (!workspace || !aligned(workspace, 256) || workspace_bytes < red.total)) return CTCT_ERR_WORKSPACE;
     a.x = logits;
     a.x_sn = row_stride;
     a.dy = dy;
@@ -603,12 +605,11 @@ int ctct_b200_adjust_backward(const void *dy, const void *logits, int64_t row_st
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     return with_type(dtype, [&](auto t) -> int {
         using T_ = decltype(t);
-        const bool some = rows > 0 && N * T > 0;
         if (some)
             if (int rc = adj_launch<T_, true>(a, vec, flat, N, packed_rows >= 0 && dx, st)) return rc;
-        if (!dbias || (direct && some) || red.outer == 0) return CTCT_OK;
-        float *parts = static_cast<float *>(workspace), *runs = some ? parts + red.parts / 4 : nullptr;
-        ReduceArgs r{parts, dbias, a.bias_f32, some ? red.P : 0, red.C};   // no row: zeros
+        if (!dbias || (direct && sums) || red.outer == 0) return CTCT_OK;
+        float *parts = static_cast<float *>(workspace), *runs = sums ? parts + red.parts / 4 : nullptr;
+        ReduceArgs r{parts, dbias, a.bias_f32, sums ? red.P : 0, red.C};   // no row: zeros
         auto few = [&](const ReduceArgs &r) {
             const int64_t blocks = ceil_div(red.outer * r.C, r.C % 4 == 0 ? 1024 : 256);
             if (blocks > kMaxGrid) return static_cast<int>(CTCT_ERR_UNSUPPORTED);
