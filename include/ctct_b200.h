@@ -462,7 +462,7 @@ int ctct_b200_layer_norm_backward(const void *dy, int64_t dy_stride, const void 
  *     want_grad only the packed layout needs it (0 bytes otherwise: may be NULL)
  * Lengths outside [0, T] and [0, U1 - 1] are clamped.  H up to CTCT_MAX_JOINT_H.
  * Backward: dy of y's shape, contiguous (its padding is not read); df (N,T,H), dg (N,U1,H) contiguous, of `dtype`,
- * zeros where no valid row is; dweight, dbias (H); each may be NULL.
+ * zeros where no valid row is, 16-byte aligned; dweight, dbias (H); each may be NULL.
  */
 #define CTCT_MAX_JOINT_H 8192
 size_t ctct_b200_joint_norm_saved_bytes(int64_t N, int64_t T, int64_t U1, int64_t packed_rows, int want_grad);
@@ -490,7 +490,7 @@ int ctct_b200_joint_norm_backward(const void *dy, const void *f, int64_t f_sn, i
  *     of `dtype`.  allowed: bit v % 32 of word v / 32, rows of ceil(V / 32) words
  *   repetition > 0, presence, frequency: for all rows, unless the pointer to (N) floats of the same name is given
  * Masked places are -inf whatever stood there.  Backward: dx (shape and type of out) and dbias (shape and type of
- * bias), each may be NULL; `logits` is read only where a repeated token is scaled (NULL if repetition is 1 for all
+ * bias, 16-byte aligned), each may be NULL; `logits` is read only where a repeated token is scaled (NULL if repetition is 1 for all
  * rows); dy is not read in padding rows, masked places get zero.  workspace: ctct_b200_adjust_workspace_bytes, for dbias only.
  */
 size_t ctct_b200_adjust_workspace_bytes(int64_t N, int64_t T, int64_t U1, int64_t V, int dtype, int packed, int bias_kind);

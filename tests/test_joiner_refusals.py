@@ -107,3 +107,29 @@ def test_adjust_entry_points_refuse_bad_arguments(lib):
         args = list(ok)
         args[i] = bad
         assert lib.ctct_b200_adjust_backward(*args) == rc, (i, bad)
+
+
+def test_frames_near_the_end_of_32_bits_are_refused(lib):
+    """Frame counters step past the last frame by up to a block's share: that must not wrap."""
+    p = 4096
+    for T in (2 ** 31 - 1, 2 ** 31 - 4096):
+        assert lib.ctct_b200_adjust_forward(p, 0, 0, None, 0, None, None, None, 1, T, 1, 1, -1, None, None, 0, 1, None, 0, 1.0, 0.0, 0.0,
+                                            None, None, None, p, None) == -1
+        assert lib.ctct_b200_adjust_workspace_bytes(1, T, 1, 1, 0, 0, 1) == 0
+        assert lib.ctct_b200_joint_norm_forward(p, T, 1, p, 1, 1, 0, None, None, 1, T, 1, 1, -1, None, None, 1, 1e-5, p, 0, None, 0,
+                                                None) == -1
+        assert lib.ctct_b200_joint_norm_workspace_bytes(1, T, 1, 1, 0) == 0
+
+
+def test_gradients_that_are_not_aligned_are_refused(lib):
+    """Sums are stored as vectors."""
+    p = 4096
+    ok = [p, p, 24, 8, p, 32, 8, 0, p, p, 2, 3, 4, 8, -1, p, 1, p, 1 << 20, p, p, p, p, p, 1 << 24, None]
+    for i in (19, 20):
+        args = list(ok)
+        args[i] = p + 4
+        assert lib.ctct_b200_joint_norm_backward(*args) == -1
+    ok = [p, p, 0, 0, p, 3, None, None, None, 2, 3, 4, 8, -1, None, 1, 1, None, 0, 1.3, None, p, p, p, 1 << 20, None]
+    args = list(ok)
+    args[22] = p + 4
+    assert lib.ctct_b200_adjust_backward(*args) == -1

@@ -30,6 +30,7 @@ int with_type(int dtype, F &&fn) {
 }
 
 constexpr int64_t kMaxGrid = 0x7fffffff;
+constexpr int64_t kMaxRun = (int64_t(1) << 31) - 4096;  // frames, contexts: loops step past the end by a block's share
 constexpr int kSms = 148;  // SMs of a B200: grids and workspaces are sized by it
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -159,8 +160,8 @@ bool jn_grad_geom(int64_t N, int64_t T, int64_t U1, int64_t H, int dtype, JnGeom
     return g->blocks <= kMaxGrid;
 }
 bool jn_dims_ok(int64_t N, int64_t T, int64_t U1, int64_t H) {
-    return N >= 0 && N <= 65535 && T >= 0 && U1 >= 1 && H >= 1 && H < (int64_t(1) << 31) && T * U1 < (int64_t(1) << 31) &&
-           N * T < (int64_t(1) << 31) && N * U1 < (int64_t(1) << 31) && N * T * U1 < (int64_t(1) << 38);
+    return N >= 0 && N <= 65535 && T >= 0 && U1 >= 1 && H >= 1 && H < (int64_t(1) << 31) && T < kMaxRun && U1 < kMaxRun &&
+           T * U1 < (int64_t(1) << 31) && N * T < (int64_t(1) << 31) && N * U1 < (int64_t(1) << 31) && N * T * U1 < (int64_t(1) << 38);
 }
 struct JnSaved {
     size_t cu, fm, gm, rstd, total;
@@ -258,7 +259,7 @@ AdjReduce adj_reduce(int64_t N, int64_t T, int64_t U1, int64_t V, int dtype, boo
 }
 bool adj_dims_ok(int64_t N, int64_t T, int64_t U1, int64_t V) {
     return N >= 0 && N <= kMaxGrid && T >= 0 && U1 >= 1 && V >= 1 && U1 < (int64_t(1) << 31) && V < (int64_t(1) << 31) &&
-           T < (int64_t(1) << 31) && U1 * V < (int64_t(1) << 31) - 4096;
+           T < kMaxRun && U1 * V < kMaxRun;
 }
 // `vec`: rows are whole vectors; `flat`: they are not, but the tensors begin with one and their rows follow one another
 template <typename T, bool GRAD>
@@ -409,6 +410,7 @@ int ctct_b200_joint_norm_backward(const void *dy, const void *f, int64_t f_sn, i
     if (packed && (!lx || !ly) && N > 0) return CTCT_ERR_ARG;
     JnGeom geo;
     if (!jn_grad_geom(N, T, U1, H, dtype, &geo)) return CTCT_ERR_UNSUPPORTED;
+    if (!aligned(df, 16) || !aligned(dg, 16)) return CTCT_ERR_ARG;   // their sums are stored as vectors
     const JnSaved sv = jn_saved(N, T, U1, packed_rows, 1);
     const JnWs ws = jn_ws(N, T, U1, H, geo);
     if (rows > 0 && (!dy || (N > 0 && T > 0 && (!f || !g)))) return CTCT_ERR_ARG;
@@ -583,6 +585,7 @@ int ctct_b200_adjust_backward(const void *dy, const void *logits, int64_t row_st
     const AdjCall c{tokens, tokens_lengths, tokens_pitch, lx, ly, N, T, U1, V, packed_rows, cu_rows, nullptr, bias_kind, bias_f32,
                     allowed, mask_kind, repetition, 0.0f, 0.0f, repetition_n, nullptr, nullptr};
     if (int rc = adj_fill(c, dtype, false, &a)) return rc;
+    if (!aligned(dbias, 16)) return CTCT_ERR_ARG;   // its sums are stored as vectors
     if ((dbias && bias_kind == 0) || row_stride < 0 || (row_stride > 0 && (T != 1 || U1 != 1 || packed_rows >= 0))) return CTCT_ERR_ARG;
     const int64_t rows = packed_rows >= 0 ? packed_rows : N * T * U1;
     const AdjReduce red = adj_reduce(N, T, U1, V, dtype, packed_rows >= 0, bias_kind);
