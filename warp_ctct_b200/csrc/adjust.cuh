@@ -12,7 +12,7 @@
 // What is done to an element depends on (n,u,v), not on the frame: a thread owns VE neighbouring elements of
 // the U1 x V plane of an utterance, keeps what is added to them and two bits each in registers, and walks over
 // frames, so that the passes are one streaming read and one streaming write of the rows (HBM-bound) and histories,
-// bias and mask are read once per block.  Histories are counted by the whole block into shared memory, integers, so
+// bias and mask are read once per block: 6.2 TB/s forward at 32x256x65x512 f32 (258 us).  Histories are counted by the whole block into shared memory, integers, so
 // the order of the atomic additions does not matter.  Outputs that are masked are selected, not
 // multiplied: NaN and infinities in masked places do not come through.
 #pragma once
@@ -53,8 +53,8 @@ struct AdjArgs {
 
 // A thread's elements: NV chunks of VE neighbours, threads * VE apart.  STEP: one row per n (T = U1 = 1), without the
 // walk over frames and with more elements per thread, since there the set-up of a block is most of its work.
-// Four blocks of 256 threads on an SM (64 registers): with three the f32 step over 1.1 GB took 396 us
-// backward instead of 338.
+// Four blocks of 256 threads on an SM (64 registers).  Three or four make little difference: forward and backward 555 and 558
+// us at 32x256x65x512 f32, 729 and 717 at 16x512x129x1024 fp16.
 template <typename T, int VE, int NV, bool GRAD, bool STEP>
 __global__ void __launch_bounds__(ADJ_THREADS, 4) k_adjust(const AdjArgs a) {
     constexpr int NE = VE * NV, UNROLL = STEP ? 1 : ADJ_UNROLL;
@@ -257,8 +257,8 @@ __global__ void __launch_bounds__(ADJ_THREADS, 4) k_adjust(const AdjArgs a) {
 // begins somewhere inside a vector: a thread owns one aligned vector of it, wherever that stands against rows.  The run
 // begins at the same place for frames that are a vector's number of elements apart, so a block's frames are that far
 // apart, and what is added to an element stays in its thread.  Only the two ends of a plane are accessed
-// element by element.  (With 2-byte accesses the f32-free step over 32x256x65x511 bf16 took 1146 us backward and 416
-// forward; whole rows of 512 take 261 and 193.)
+// element by element.  32x256x65x511 bf16, all rows valid: 414 us backward and 305 forward, with 2-byte accesses 1146 and
+// 416; rows of 512, which are whole vectors, take 277 and 206.
 template <typename T, bool GRAD>
 __global__ void __launch_bounds__(ADJ_THREADS, 4) k_adjust_flat(const AdjArgs a) {
     constexpr int VE = 16 / static_cast<int>(sizeof(T));

@@ -4,7 +4,7 @@
 //   q = w dy,  dx = r (q - mean(q) - xh mean(q xh)),  dw = sum over rows of dy xh,  db = sum over rows of dy
 //
 // A row stays in registers between the two sums and the output, so every element is read once and
-// written once: the bound is HBM traffic.  The variance is the mean of squared deviations (a second
+// written once: the bound is HBM traffic (16000 x 4096 f32: 6.2 TB/s forward, 85 us; 5.6 backward, 140 us).  The variance is the mean of squared deviations (a second
 // pass over the registers), not a difference of moments, so a large common offset costs no digits.
 // The weight's and the bias's gradient are accumulated in registers over all rows that a block takes
 // (a thread owns its columns), leave as one float32 partial row per block, and are added up in a fixed order.
@@ -46,7 +46,7 @@ constexpr int LN_WIDE_THREADS = 512; // largest block that shares one row
 // of 16-byte vectors, one behind the other: chunks are the aligned vectors that a row lies in, so its first column stands
 // `shift` elements inside a vector.  A block's rows are a multiple of a vector's elements apart, so the shift
 // is the block's and a thread keeps its columns; only the row's two ends are accessed element by element.  (With
-// 2-byte accesses 16000 rows of 1023 bf16 took 37 us forward and 148 backward; rows of 1024 take 17 and 30.)
+// 2-byte accesses 16000 rows of 1023 bf16 took 37 us forward and 148 backward, so 33 and 48; rows of 1024 take 14 and 29.)
 template <typename T, int VE, int NV, bool ODD>
 struct LnCols {
     int col[NV];
